@@ -4,6 +4,15 @@ attention-chain GPU ops behind the reference's own ``galois_*`` op API.
 Importing the package loads ``libgalois_b200.so``; there is no CPU fallback.
 """
 from ._lib import LIB_PATH, lib  # noqa: F401  (raises if the library is missing)
+from .cache import (  # noqa: F401
+    CacheQ8,
+    galois_cache_append,
+    galois_cache_attention,
+    galois_cache_attention_workspace,
+    galois_cache_evict,
+    galois_cache_read,
+    galois_prompt_attention,
+)
 from .op import (  # noqa: F401
     RopeCustomOption,
     UnaryOp,

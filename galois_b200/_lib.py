@@ -48,8 +48,15 @@ class GaloisDecodeShape(C.Structure):
                 ("eps", C.c_float), ("rope_freq_base", C.c_float), ("rope_freq_scale", C.c_float)]
 
 
+class GaloisCacheQ8(C.Structure):
+    """``galois_b200_cache_q8``: the parts and the layout of an 8-bit key/value cache."""
+
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("qd", GaloisDim), ("sd", GaloisDim)]
+
+
 _P, _F, _I, _I64, _SZ = C.c_void_p, C.c_float, C.c_int, C.c_int64, C.c_size_t
 _DP = C.POINTER(GaloisDim)
+_CQ = C.POINTER(GaloisCacheQ8)
 
 # name -> (argtypes, restype); must list every function include/galois_b200.h declares
 SIGNATURES = {
@@ -108,6 +115,15 @@ SIGNATURES = {
     "galois_b200_decode_workspace_bytes": ([_P, C.POINTER(GaloisDecodeShape), C.POINTER(_SZ)], _I),
     "galois_b200_decode_layers_f32": ([_P, C.POINTER(GaloisDecodeShape), C.POINTER(GaloisDecodeLayer), _I, _P, _P, _P, _P, _SZ], _I),
     "galois_b200_decode_attention_f32": ([_P, C.POINTER(GaloisDecodeShape), C.POINTER(GaloisDecodeLayer), _P, _P, _P, _P, _SZ], _I),
+    "galois_b200_prompt_attention_f16": ([_P, _P, _DP, _P, _DP, _P, _DP, _P, _P, _I, _P, _DP, _F], _I),
+    "galois_b200_prompt_attention_f16_f32": ([_P, _P, _DP, _P, _DP, _P, _DP, _P, _P, _I, _P, _DP, _F], _I),
+    "galois_b200_cache_append_f32": ([_P, _CQ, _P, _DP, _P, _DP, _P, _P, _I], _I),
+    "galois_b200_cache_append_f16": ([_P, _CQ, _P, _DP, _P, _DP, _P, _P, _I], _I),
+    "galois_b200_cache_read_f32": ([_P, _CQ, _P, _P, _I, _P, _DP, _P, _DP], _I),
+    "galois_b200_cache_read_f16": ([_P, _CQ, _P, _P, _I, _P, _DP, _P, _DP], _I),
+    "galois_b200_cache_attention_workspace_bytes": ([_P, _CQ, _I, _I, C.POINTER(_SZ)], _I),
+    "galois_b200_cache_attention_f32": ([_P, _P, _DP, _CQ, _P, _P, _DP, _F, _P, _DP, _P, _DP, _P, _SZ], _I),
+    "galois_b200_cache_evict": ([_P, _CQ, _P, _P, _DP, _I, _CQ, _P, _P, _DP, _P, _DP], _I),
     "galois_b200_shard_rows": ([_I64, _I, _I, C.POINTER(_I64), C.POINTER(_I64)], _I),
     "galois_b200_ipc_export": ([_P, _P, C.c_char_p], _I),
     "galois_b200_ipc_import": ([_P, C.c_char_p, C.POINTER(_P)], _I),

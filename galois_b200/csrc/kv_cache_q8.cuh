@@ -1,0 +1,97 @@
+// The 8-bit key/value cache: what its operators share (argument checks on the host, the rounding to whole
+// numbers and the look-up of packed rows on the device).
+#pragma once
+#include "common.cuh"
+
+#define GB_CACHE_BLOCK 32  // tokens of one head that share a scale
+
+// Makes the context's device current for the calls of one entry point and puts the caller's back.
+struct gb_on_device {
+    int before = -1;
+    explicit gb_on_device(const galois_b200_ctx* ctx) {
+        if (cudaGetDevice(&before) == cudaSuccess && before != ctx->ordinal)
+            cudaSetDevice(ctx->ordinal);
+        else
+            before = -1;
+    }
+    ~gb_on_device() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
+// Bytes from the first to behind the last element of a tensor (0 if it has none).
+static inline size_t gb_span(const galois_dim* d, size_t elem) {
+    size_t last = 0;
+    for (int i = 0; i < 4; i++) {
+        if (d->ne[i] <= 0) return 0;
+        last += (size_t)(d->ne[i] - 1) * (size_t)d->nb[i];
+    }
+    return (last + 1) * elem;
+}
+static inline bool gb_overlap(const void* a, size_t an, const void* b, size_t bn) {
+    return an && bn && (uintptr_t)a < (uintptr_t)b + bn && (uintptr_t)b < (uintptr_t)a + an;
+}
+// No two elements at one address: sorted by stride, each dimension steps over all of the smaller ones.
+static inline bool gb_injective(const galois_dim* d) {
+    int64_t span = 1;
+    bool used[4] = {false, false, false, false};
+    for (int k = 0; k < 4; k++) {
+        int at = -1;
+        for (int i = 0; i < 4; i++)
+            if (!used[i] && d->ne[i] > 1 && (at < 0 || d->nb[i] < d->nb[at])) at = i;
+        if (at < 0) return true;
+        used[at] = true;
+        if (d->nb[at] < span) return false;
+        span = (d->ne[at] - 1) * d->nb[at] + span;
+    }
+    return true;
+}
+
+// Strides of a {head_dim, heads, tokens} operand and of the cache, in elements.
+struct gb_cache_view {
+    int8_t *k, *v;
+    float *ks, *vs;
+    int64_t tok, head, seq;     // strides of k and v
+    int64_t s_head, s_seq;      // strides of the scales
+    int ctx, kv_heads, seqs, head_dim;
+};
+// 0 and *out filled, or a failure of `what`.
+int gb_check_cache(galois_b200_ctx* ctx, const char* what, const galois_b200_cache_q8* cache, gb_cache_view* out);
+
+#ifdef __CUDACC__
+// The sequence that packed row t belongs to: the number of starts[1..n] that are <= t.  Called by a whole warp;
+// the loads of a warp are independent of each other, so a batch of 32 sequences costs one trip to memory where a
+// binary search costs five.
+__device__ __forceinline__ int gb_find_seq(const int32_t* __restrict__ starts, int n, int t) {
+    int c = 0;
+    for (int i = threadIdx.x & 31; i < n; i += 32) c += starts[i + 1] <= t;
+    return __reduce_add_sync(0xffffffffu, c);
+}
+
+// round-half-even of the exact quotient x / d, limited to -127..127.  x * (1 / d) is off by at most two units of the
+// last place, so its rounding is wrong only next to a border k + 1/2; the sign of x - (k + 1/2) d, which one fused
+// multiply-add gives exactly (d is not below 2^-100), decides there.
+__device__ __forceinline__ int gb_q8_round(float x, float d, float rd) {
+    float q = rintf(__fmul_rn(x, rd));
+    const float lo = fmaf(-(q - 0.5f), d, x), hi = fmaf(-(q + 0.5f), d, x);
+    const bool odd = ((int)q) & 1;
+    if (lo < 0.0f || (lo == 0.0f && odd)) q -= 1.0f;
+    else if (hi > 0.0f || (hi == 0.0f && odd)) q += 1.0f;
+    return max(-127, min(127, (int)q));
+}
+// The same of q0 * d0 / d for a whole number that moves to a larger scale; r = d0 / d rounded.  The product has 32
+// bits, so next to a border the two sides are compared in 64 bits, where both are exact.
+__device__ __forceinline__ int gb_q8_rescale(int q0, float d0, float d, float r) {
+    const float t = __fmul_rn((float)q0, r);
+    float q = rintf(t);
+    if (fabsf(t - q) > 0.5f - 0x1p-15f) {
+        const double x = (double)q0 * (double)d0;
+        const double lo = x - ((double)q - 0.5) * (double)d, hi = x - ((double)q + 0.5) * (double)d;
+        const bool odd = ((int)q) & 1;
+        if (lo < 0.0 || (lo == 0.0 && odd)) q -= 1.0f;
+        else if (hi > 0.0 || (hi == 0.0 && odd)) q += 1.0f;
+    }
+    return max(-127, min(127, (int)q));
+}
+__device__ __forceinline__ int gb_sx(uint32_t w, int i) { return (int)(int8_t)(w >> (8 * i)); }
+#endif

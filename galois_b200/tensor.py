@@ -34,13 +34,14 @@ class GGmlType(enum.IntEnum):
     F16 = 1
     Q4_0 = 2
     Q6K = 14
+    I8 = 16
     I32 = 18
 
 
 # elements per block and bytes per block (GS_BLCK_SIZE / GS_TYPE_SIZE, src/lib.rs:340-375)
-BLCK_SIZE = {GGmlType.F32: 1, GGmlType.F16: 1, GGmlType.Q4_0: QK4_0, GGmlType.Q6K: 256, GGmlType.I32: 1}
-TYPE_SIZE = {GGmlType.F32: 4, GGmlType.F16: 2, GGmlType.Q4_0: 18, GGmlType.Q6K: 210, GGmlType.I32: 4}
-_NP_DTYPE = {GGmlType.F32: np.float32, GGmlType.F16: np.float16, GGmlType.I32: np.int32}
+BLCK_SIZE = {GGmlType.F32: 1, GGmlType.F16: 1, GGmlType.Q4_0: QK4_0, GGmlType.Q6K: 256, GGmlType.I8: 1, GGmlType.I32: 1}
+TYPE_SIZE = {GGmlType.F32: 4, GGmlType.F16: 2, GGmlType.Q4_0: 18, GGmlType.Q6K: 210, GGmlType.I8: 1, GGmlType.I32: 4}
+_NP_DTYPE = {GGmlType.F32: np.float32, GGmlType.F16: np.float16, GGmlType.I8: np.int8, GGmlType.I32: np.int32}
 
 
 @dataclass
@@ -193,6 +194,7 @@ class Tensor:
         self.storage = storage
         self.device = device
         self.offset = offset  # in elements (blocks for Q4_0) from the start of `storage`
+        self._c_dim = None
 
     # ---- constructors ------------------------------------------------
     @staticmethod
@@ -227,7 +229,7 @@ class Tensor:
         if device.is_gpu:
             import torch
 
-            tdt = {GGmlType.F32: torch.float32, GGmlType.F16: torch.float16, GGmlType.I32: torch.int32}.get(dtype)
+            tdt = {GGmlType.F32: torch.float32, GGmlType.F16: torch.float16, GGmlType.I8: torch.int8, GGmlType.I32: torch.int32}.get(dtype)
             if dtype in (GGmlType.Q4_0, GGmlType.Q6K):
                 st = torch.zeros(n * TYPE_SIZE[dtype], dtype=torch.uint8, device=device.gpu.torch_device)
             else:
@@ -250,6 +252,12 @@ class Tensor:
     # ---- accessors -----------------------------------------------------
     def dim(self) -> Dim:
         return self._dim
+
+    def c_dim(self):
+        """The C form of ``dim()`` by reference, built once: a tensor's shape and strides do not change."""
+        if self._c_dim is None:
+            self._c_dim = self._dim.c_struct()
+        return C.byref(self._c_dim)
 
     def shape(self):
         return self._dim.shape[: self._dim.n_dims]

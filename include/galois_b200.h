@@ -428,6 +428,77 @@ int galois_b200_decode_layers_f32(galois_b200_ctx* ctx, const galois_b200_decode
 int galois_b200_decode_attention_f32(galois_b200_ctx* ctx, const galois_b200_decode_shape* shape, const galois_b200_decode_layer* layer,
                                      const float* qkv, const int32_t* pos, float* context, void* workspace, size_t workspace_bytes);
 
+/* ---- prompts, and a key/value cache in 8 bits --------------------------- */
+
+/* No counterpart in the reference, whose attention is composed from mat-muls and soft_max over an F16 cache
+ * (src/op.rs:3093-3111, 3216-3230).  The entry points below serve batches of sequences with grouped heads
+ * (`heads` query heads over `kv_heads` key/value heads, heads % kv_heads == 0, consecutive heads share), head_dim
+ * 64 or 128.  Rows (head_dim numbers) are contiguous and 16-byte aligned, other strides free; destinations may not
+ * overlap operands except where stated.  Packed rows: tokens starts[s] <= t < starts[s + 1] of a {head_dim, heads,
+ * tokens} tensor belong to sequence s (i32 on the device, nseq + 1 of them, ascending); rows behind the last
+ * sequence are neither read nor written.  Starts, positions and lengths out of range: that sequence's part is left
+ * out and the next synchronising call returns GALOIS_B200_E_BADARG. */
+
+/* out_i = sum_j softmax_j(scale * q_i . k_j) v_j, where query i of a sequence with nq queries and nk keys sees the
+ * keys j <= i + nk - nq (causal; a prompt that continues nk - nq earlier tokens).  Queries that see no key give
+ * zeros; keys that a query does not see do not touch its result, whatever they hold.  q, dst {head_dim, heads,
+ * tokens}; k, v {head_dim, kv_heads, tokens}; q_starts and k_starts may be the same array.  q, k, v are F16, dst F16
+ * or f32; logits, sums and the running maximum are f32, the probabilities are rounded to F16 for the second product
+ * as galois_matmul rounds its f32 operand for an F16 one. */
+int galois_b200_prompt_attention_f16(galois_b200_ctx* ctx, const void* q, const galois_dim* qd, const void* k, const galois_dim* kd, const void* v,
+                                     const galois_dim* vd, const int32_t* q_starts, const int32_t* k_starts, int nseq, void* dst,
+                                     const galois_dim* dd, float scale);
+int galois_b200_prompt_attention_f16_f32(galois_b200_ctx* ctx, const void* q, const galois_dim* qd, const void* k, const galois_dim* kd, const void* v,
+                                         const galois_dim* vd, const int32_t* q_starts, const int32_t* k_starts, int nseq, float* dst,
+                                         const galois_dim* dd, float scale);
+
+/* A cache of `sequences` slots: row j of a head stands for k[j] * k_scale[j / 32], numbers -127..127, likewise v.
+ * Strides of qd are multiples of 16 (bytes); no two rows may overlap.  Every use names the rows that count, so a new
+ * cache needs no clearing. */
+typedef struct galois_b200_cache_q8 {
+    void *k, *v;               /* i8, both laid out as qd: {head_dim, ctx, kv_heads, sequences} */
+    float *k_scale, *v_scale;  /* both laid out as sd: {ceil(ctx / 32), kv_heads, sequences} */
+    galois_dim qd, sd;
+} galois_b200_cache_q8;
+
+/* Puts new tokens into the cache: packed row i of sequence s (k, v {head_dim, kv_heads, tokens}, f32 or F16) becomes
+ * cache row pos[s] + i of slot s.  A block of 32 rows has the scale f32(max |x| / 127) of the largest number it was
+ * given; if the block already holds rows before pos[s] and the scale has to grow, they are brought to the new one.
+ * Numbers are rounded half to even from the exact quotient x / scale.  NaN is stored as 0, infinities as the largest
+ * finite number; a scale below 2^-100 as 0, and its block as zeros.  Rows at and behind pos[s] that the block held
+ * before do not count. */
+int galois_b200_cache_append_f32(galois_b200_ctx* ctx, const galois_b200_cache_q8* cache, const float* k, const galois_dim* kd, const float* v,
+                                 const galois_dim* vd, const int32_t* starts, const int32_t* pos, int nseq);
+int galois_b200_cache_append_f16(galois_b200_ctx* ctx, const galois_b200_cache_q8* cache, const void* k, const galois_dim* kd, const void* v,
+                                 const galois_dim* vd, const int32_t* starts, const int32_t* pos, int nseq);
+/* The inverse: packed row i of sequence s of k and v receives the values of cache row pos[s] + i of slot s (exact in
+ * f32, rounded to nearest even in F16), e.g. the earlier tokens that a prompt continues. */
+int galois_b200_cache_read_f32(galois_b200_ctx* ctx, const galois_b200_cache_q8* cache, const int32_t* starts, const int32_t* pos, int nseq,
+                               float* k, const galois_dim* kd, float* v, const galois_dim* vd);
+int galois_b200_cache_read_f16(galois_b200_ctx* ctx, const galois_b200_cache_q8* cache, const int32_t* starts, const int32_t* pos, int nseq,
+                               void* k, const galois_dim* kd, void* v, const galois_dim* vd);
+
+/* One new token per slot over the first lens[s] rows of its cache: out = sum_j softmax_j(scale * q . k_j) v_j; a
+ * length of 0 gives zeros.  q, dst f32 {head_dim, heads, sequences}.  With `weights` (f32 {ctx, kv_heads, sequences};
+ * NULL for none, then weights_out is NULL too) weights_out[j] = weights[j] + the sum over the group's heads of the
+ * probability of row j, for j < lens[s]; weights_out may be weights itself.  workspace:
+ * galois_b200_cache_attention_workspace_bytes(cache, heads, with_weights) bytes, 16-byte aligned, contents
+ * irrelevant; calls that may run at the same time (graphs replayed on two streams) need one each. */
+int galois_b200_cache_attention_workspace_bytes(galois_b200_ctx* ctx, const galois_b200_cache_q8* cache, int heads, int with_weights,
+                                                size_t* out_bytes);
+int galois_b200_cache_attention_f32(galois_b200_ctx* ctx, const float* q, const galois_dim* qd, const galois_b200_cache_q8* cache,
+                                    const int32_t* lens, float* dst, const galois_dim* dd, float scale, const float* weights,
+                                    const galois_dim* wd, float* weights_out, const galois_dim* wod, void* workspace, size_t workspace_bytes);
+
+/* Cuts every slot and head down to the `ctx` rows of `out`: m = min(lens[s], out ctx) rows stay, the last
+ * min(recent, m) and, of the others, those of largest weight (f32 {ctx, kv_heads, sequences}; equal weights: the
+ * lowest row first; NaN below all), in their order.  index (i32) receives their old rows, out_weights their weights
+ * (both {out ctx, kv_heads, sequences}, entries behind m are left as they were), out_lens[s] = m.  Their numbers are
+ * brought to the largest scale of each new block's rows (rounded half to even). */
+int galois_b200_cache_evict(galois_b200_ctx* ctx, const galois_b200_cache_q8* cache, const int32_t* lens, const float* weights,
+                            const galois_dim* wd, int recent, const galois_b200_cache_q8* out, int32_t* out_lens, float* out_weights,
+                            const galois_dim* owd, int32_t* index, const galois_dim* id);
+
 /* ---- row sharding across GPUs ------------------------------------------ */
 
 /* Row range [*row0, *row0 + *nrows) of an N-row weight owned by `rank` of
