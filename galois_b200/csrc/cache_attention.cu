@@ -6,54 +6,487 @@
 // 0 gives zeros.  With `weights`, weights_out[j] = weights[j] + the sum of p_j over the heads of the group.
 #include "kv_cache_q8.cuh"
 
+#include "ptx.cuh"
+#include "tma.cuh"
+
 namespace {
 
-// One CTA per (head, sequence); a warp takes every fourth row, a lane HD / 32 numbers of it.
+// What has to be read is 2 HD bytes a row and head (the arithmetic, 4 HD flops a row and query head, is far below
+// the machine's), so the kernel is built to keep HBM busy whatever the lengths are:
+//
+//  * The rows of all (sequence, key/value head) pairs form one list of 32-row blocks, which is dealt evenly to all
+//    warps of the device, each a contiguous part; a part may begin and end inside a pair.  No length is known on the
+//    host, and none makes a warp wait for another: a warp writes what it has of a pair as one piece (maximum, sum, HD
+//    numbers per head), and a second launch joins the pieces.
+//  * Each warp streams its blocks through a ring of its own in shared memory, across the borders of pairs: one TMA copy
+//    for the keys of a block and one for its values; nothing synchronises the CTA.  The logits of the next block are
+//    formed between the soft-max and the products of this one, so that a warp always has independent work to issue.
+//  * The whole numbers are exact in F16, so both products run on mma.sync m16n8k16 with f32 sums: the 16 rows are up
+//    to 8 heads of the group twice, once with the upper and once with the lower 11 bits of the f32 operand (the query,
+//    scaled to 2^7..2^8; the probability), which keeps f32's accuracy.  The order of a contraction is free, so
+//    fragments are taken as a lane's 16-byte loads give them: of the keys, lane (g, t) has numbers 16 t.. of one row; of
+//    the values, CW numbers of four rows, whose bytes are paired by permutes.  Which row and which chunk g and t stand
+//    for is chosen so that the eight lanes of a load's phase meet no bank of the swizzled tile twice.
+constexpr int WARPS = 12;
+constexpr int BLK = GB_CACHE_BLOCK;
 template <int HD>
-__global__ void __launch_bounds__(128) cache_attention_kernel(const float* __restrict__ q, int64_t q_head, int64_t q_seq, gb_cache_view c,
-                                                              const int32_t* __restrict__ lens, float* __restrict__ out, int64_t o_head, int64_t o_seq,
-                                                              int heads, float scale, float* __restrict__ stats, float* __restrict__ scores,
-                                                              int* __restrict__ status) {
+struct ring {
+    static constexpr int HALF = BLK * HD;    // bytes of a block's keys (or values)
+    static constexpr int DEPTH = HD == 128 ? 2 : 4;   // tiles of keys, and as many of values
+    static constexpr int BARS = 1024 + WARPS * 2 * DEPTH * HALF;  // offset of the barriers; 1024 to align the tiles
+    static constexpr int TOTAL = BARS + WARPS * 2 * DEPTH * 8;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float low(uint64_t a) { return __uint_as_float((uint32_t)a); }
+__device__ __forceinline__ float high(uint64_t a) { return __uint_as_float((uint32_t)(a >> 32)); }
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+    uint32_t d;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    return d;
+}
+// Two numbers as F16 pairs: the nearest, and what is left of each.
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    hi = pack_half2(a, b);
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+    lo = pack_half2(a - f.x, b - f.y);
+}
+__device__ __forceinline__ uint32_t minus_1152(uint32_t h) {  // 1024 + (q + 128) -> q, exact
+    const __half2 r = __hadd2(*reinterpret_cast<const __half2*>(&h), __half2half2(__ushort_as_half((unsigned short)0xe480)));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint4 lds128(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t at) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
+    return v;
+}
+// Where 16-byte chunk c of a block's row lies: TMA's swizzle over rows of 128 or 64 bytes.
+template <int HD>
+__device__ __forceinline__ uint32_t tile_at(int row, int c) {
+    return HD == 128 ? (uint32_t)(row * 128 + ((c ^ (row & 7)) << 4)) : (uint32_t)(row * 64 + ((c ^ ((row >> 1) & 3)) << 4));
+}
+// The row of a block that column n of the n-tile j of logits stands for.
+template <int HD>
+__device__ __forceinline__ int row_of(int j, int n) {
+    return 8 * j + (HD == 128 ? (n >> 1) + 4 * (n & 1) : n);
+}
+
+__device__ __forceinline__ int checked_len(int n, int ctx) { return n < 0 || n > ctx ? 0 : n; }
+
+// How the list of blocks is dealt: `total` blocks over `warps` contiguous parts, none of them empty.
+struct deal {
+    int64_t total;
+    int warps;
+    __device__ deal(int64_t n, int most) : total(n), warps((int)min(n, (int64_t)most)) {}
+    __device__ int64_t begin(int w) const { return (int64_t)w * total / warps; }
+    __device__ int owner(int64_t b) const { return (int)(((b + 1) * warps - 1) / total); }
+};
+
+// Sum over the warp of `per` x the blocks of sequences [0, n).
+__device__ __forceinline__ int64_t count_blocks(const int32_t* __restrict__ lens, int n, int ctx, int per) {
+    int64_t c = 0;
+    for (int i = threadIdx.x & 31; i < n; i += 32) c += (checked_len(lens[i], ctx) + BLK - 1) / BLK;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
+    return c * per;
+}
+
+// A place in the list: block `blk` of `blocks` of pair `inner` of sequence `seq`.
+struct cursor {
+    int seq, inner, blk, blocks, len;
+    __device__ __forceinline__ void next_seq(const int32_t* __restrict__ lens, int nseq, int ctx) {
+        do {
+            seq++;
+            len = seq < nseq ? checked_len(lens[seq], ctx) : 1;
+        } while (len == 0);
+        blocks = (len + BLK - 1) / BLK;
+    }
+    __device__ __forceinline__ void advance(const int32_t* __restrict__ lens, int nseq, int ctx, int per) {
+        if (++blk < blocks) return;
+        blk = 0;
+        if (++inner < per) return;
+        inner = 0;
+        next_seq(lens, nseq, ctx);
+    }
+};
+
+struct step_args {
+    const float* q;
+    int64_t q_head, q_seq;
+    gb_cache_view c;
+    const int32_t* lens;
+    int group, tiles;  // query heads per key/value head; tiles of 8 of them
+    int rows;          // min(8, group): heads that a piece holds
+    float scale;
+    float *acc, *stats;  // pieces: [piece][rows][HD], [piece][rows][2]
+    float* scores;       // [seq][heads][ctx] base-2 logits, or null
+    int* status;
+};
+
+template <int HD>
+__global__ void __launch_bounds__(WARPS * 32, 1)
+    cache_attention_kernel(const step_args p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    constexpr int CW = HD / 8, NW = CW / 4, KS = HD / 16;  // bytes of a value row per lane, words of them, steps over head_dim
+    constexpr int DEPTH = ring<HD>::DEPTH;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + ring<HD>::BARS) + warp * 2 * DEPTH;  // of the keys' tiles, then of the values'
+    if (lane == 0) {
+        tma_prefetch_map(&k_map);
+        tma_prefetch_map(&v_map);
+        for (int i = 0; i < 2 * DEPTH; i++) mbar_init(bars + i, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
     gb_pdl_entry();
-    constexpr int E = HD / 32;
-    __shared__ float sm[4], sl[4], so[4][HD];
-    const int h = blockIdx.x, s = blockIdx.y, kh = h / (heads / c.kv_heads), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int n = lens[s];
-    if (n < 0 || n > c.ctx) {
-        if (threadIdx.x == 0) *status = GALOIS_B200_E_BADARG;
-        n = 0;
+    const gb_cache_view& c = p.c;
+    const int per = c.kv_heads * p.tiles, heads = c.kv_heads * p.group;
+    const deal D(count_blocks(p.lens, c.seqs, c.ctx, per), (int)gridDim.x * WARPS);
+    if (blockIdx.x == 0 && warp == 0)
+        for (int i = lane; i < c.seqs; i += 32)
+            if (p.lens[i] < 0 || p.lens[i] > c.ctx) *p.status = GALOIS_B200_E_BADARG;
+    const int w = warp * (int)gridDim.x + (int)blockIdx.x;  // parts of neighbours lie on different SMs
+    if (w >= D.warps) return;
+    const int64_t b0 = D.begin(w), b1 = D.begin(w + 1);
+    // the place of block b0
+    cursor at{-1, 0, 0, 0, 0};
+    {
+        int64_t before = 0;
+        for (int s0 = 0;; s0 += 32) {
+            const int n = s0 + lane < c.seqs ? checked_len(p.lens[s0 + lane], c.ctx) : 0;
+            int64_t mine = (int64_t)((n + BLK - 1) / BLK) * per, upto = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t y = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += y;
+            }
+            const uint32_t past = __ballot_sync(0xffffffffu, before + upto > b0);
+            if (past) {
+                const int l = __ffs(past) - 1;
+                const int64_t off = b0 - before - (__shfl_sync(0xffffffffu, upto, l) - __shfl_sync(0xffffffffu, mine, l));
+                at.seq = s0 + l;
+                at.len = __shfl_sync(0xffffffffu, n, l);
+                at.blocks = (at.len + BLK - 1) / BLK;
+                at.inner = (int)(off / at.blocks);
+                at.blk = (int)(off % at.blocks);
+                break;
+            }
+            before += __shfl_sync(0xffffffffu, upto, 31);
+        }
     }
-    float qr[E], o[E], m = -INFINITY, l = 0.0f;
+    const uint32_t base = ((smem_u32(smem) + 1023u) & ~1023u) + (uint32_t)(warp * 2 * DEPTH * ring<HD>::HALF);
+    // Keys are wanted one block earlier than values: the place of the newest keys is kept for the values' next copy.
+    cursor ahead = at;
+    int last_blk = 0, last_kh = 0, last_seq = 0;
+    int64_t fetched = b0;  // blocks whose keys have been asked for
+    // the scales of blocks b.., in the ring's order
+    float2 scales[DEPTH + 1];
+    auto fetch_keys = [&](int slot) -> float2 {
+        last_blk = ahead.blk, last_kh = ahead.inner / p.tiles, last_seq = ahead.seq;
+        const int64_t sat = last_kh * c.s_head + last_seq * c.s_seq + last_blk;
+        const float2 sc = make_float2(__ldg(c.ks + sat), __ldg(c.vs + sat));
+        if (lane == 0) {
+            mbar_expect_tx(bars + slot, ring<HD>::HALF);
+            tma_load_4d(base + (uint32_t)(slot * ring<HD>::HALF), &k_map, 0, last_blk * BLK, last_kh, last_seq, bars + slot);
+        }
+        ahead.advance(p.lens, c.seqs, c.ctx, per);
+        fetched++;
+        return sc;
+    };
+    auto fetch_values = [&](int slot) {
+        if (lane == 0) {
+            mbar_expect_tx(bars + DEPTH + slot, ring<HD>::HALF);
+            tma_load_4d(base + (uint32_t)((DEPTH + slot) * ring<HD>::HALF), &v_map, 0, last_blk * BLK, last_kh, last_seq, bars + DEPTH + slot);
+        }
+    };
 #pragma unroll
-    for (int e = 0; e < E; e++) qr[e] = q[h * q_head + s * q_seq + lane * E + e] * scale, o[e] = 0.0f;
-    for (int j = warp; j < n; j += 4) {
-        const int64_t at = kh * c.head + s * c.seq + j * c.tok + lane * E, sat = kh * c.s_head + s * c.s_seq + j / GB_CACHE_BLOCK;
-        float x = 0.0f;
-#pragma unroll
-        for (int e = 0; e < E; e++) x = fmaf(qr[e], (float)c.k[at + e], x);
-        x = gb_warp_sum(x) * c.ks[sat];
-        if (scores && lane == 0) scores[((int64_t)s * heads + h) * c.ctx + j] = x;
-        const float top = fmaxf(m, x), keep = m == -INFINITY ? 0.0f : expf(m - top), p = x == -INFINITY ? 0.0f : expf(x - top);
-        m = top;
-        l = l * keep + p;
-#pragma unroll
-        for (int e = 0; e < E; e++) o[e] = fmaf(p * c.vs[sat], (float)c.v[at + e], o[e] * keep);
+    for (int i = 0; i < DEPTH; i++) {
+        scales[i] = make_float2(0.f, 0.f);
+        if (fetched < b1) scales[i] = fetch_keys(i), fetch_values(i);
     }
-    if (lane == 0) sm[warp] = m, sl[warp] = l;
+    scales[DEPTH] = make_float2(0.f, 0.f);
+    uint32_t phases = 0;  // bit i: parity that barrier i completes next
+    auto wait = [&](int bar) {
+        const bool ok = mbar_wait_bounded(bars + bar, (phases >> bar) & 1);
+        phases ^= 1u << bar;
+        return __all_sync(0xffffffffu, ok);
+    };
+
+    uint32_t qa[KS][4];
+    float factor = 0.0f;
+    // The query of the pair at `at`: lane (g, t) holds numbers 16 (t + 4 i) + 4 j.. of head g, times the power of two that
+    // brings the largest to 2^7..2^8, as two F16 each.
+    auto load_query = [&]() {
+        const int head0 = at.inner / p.tiles * p.group + (at.inner % p.tiles) * 8, live = min(8, p.group - (at.inner % p.tiles) * 8);
+        float4 f[KS];
+        float top = 0.0f;
+        const float* qh = p.q + (int64_t)(head0 + g) * p.q_head + (int64_t)at.seq * p.q_seq;
 #pragma unroll
-    for (int e = 0; e < E; e++) so[warp][lane * E + e] = o[e];
-    __syncthreads();
-    const float top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-    float f[4], total = 0.0f;
+        for (int i = 0; i < KS; i++) {
+            f[i] = g < live ? *reinterpret_cast<const float4*>(qh + 16 * (t + 4 * (i / 4)) + 4 * (i % 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            top = fmaxf(top, fmaxf(fmaxf(fabsf(f[i].x), fabsf(f[i].y)), fmaxf(fabsf(f[i].z), fabsf(f[i].w))));
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = max(-110, min(120, (int)(__float_as_uint(top) >> 23) - 127));
+        const float up = __uint_as_float((uint32_t)(127 + 7 - e) << 23);
+        factor = __uint_as_float((uint32_t)(127 - 7 + e) << 23) * p.scale * 1.4426950408889634f;
 #pragma unroll
-    for (int w = 0; w < 4; w++) f[w] = sm[w] == -INFINITY ? 0.0f : expf(sm[w] - top), total += f[w] * sl[w];
-    if (stats && threadIdx.x == 0) stats[2 * ((int64_t)s * heads + h)] = top, stats[2 * ((int64_t)s * heads + h) + 1] = total;
-    for (int e = threadIdx.x; e < HD; e += 128) {
-        float x = 0.0f;
+        for (int i = 0; i < KS; i++) {
+            split2(f[i].x * up, f[i].y * up, qa[i][0], qa[i][1]);
+            split2(f[i].z * up, f[i].w * up, qa[i][2], qa[i][3]);
+        }
+    };
+    // Base-2 logits of a block's 32 rows: lane (g, t) gets those of head g and rows row_of(j, 2 t), row_of(j, 2 t + 1).
+    auto logits = [&](int slot, float k_scale, float (&x)[4][2]) {
+        const uint32_t ks = base + (uint32_t)(slot * ring<HD>::HALF);
+        const float f = k_scale * factor;
 #pragma unroll
-        for (int w = 0; w < 4; w++)
-            if (f[w] != 0.0f) x += f[w] * so[w][e];
-        out[h * o_head + s * o_seq + e] = total == 0.0f ? 0.0f : x / total;
+        for (int j = 0; j < 4; j++) {
+            float s[KS / 4][4];
+#pragma unroll
+            for (int cc = 0; cc < KS / 4; cc++) {
+                s[cc][0] = s[cc][1] = s[cc][2] = s[cc][3] = 0.0f;
+                const uint4 kw = lds128(ks + tile_at<HD>(row_of<HD>(j, g), t + 4 * cc));
+                const uint32_t word[4] = {kw.x, kw.y, kw.z, kw.w};
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const uint32_t u = word[i] ^ 0x80808080u;
+                    mma16816(s[cc], qa[4 * cc + i][0], qa[4 * cc + i][1], qa[4 * cc + i][2], qa[4 * cc + i][3],
+                             minus_1152(__byte_perm(u, 0x64646464u, 0x4140)), minus_1152(__byte_perm(u, 0x64646464u, 0x4342)));
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                float y = s[0][e] + s[0][e + 2];
+                if constexpr (KS == 8) y += s[1][e] + s[1][e + 2];
+                x[j][e] = y * f;
+            }
+        }
+    };
+
+    uint64_t o[NW * 4];  // pairs of f32
+#pragma unroll
+    for (int i = 0; i < NW * 4; i++) o[i] = 0;
+    float m = -INFINITY, l = 0.0f, vinv = 0.0f, vtop = 0.0f;
+    float x[4][2], xn[4][2];
+    load_query();
+    int slot = 0;
+    bool fine = wait(0);
+    logits(0, scales[0].x, x);
+    __syncwarp();
+    bool more = fetched < b1;  // the block behind the ring exists: its keys now, its values when block b's are used
+    if (more) scales[DEPTH] = fetch_keys(0);
+    for (int64_t b = b0; b < b1 && fine; b++) {
+        const int next = slot + 1 == DEPTH ? 0 : slot + 1;
+        if (b + 1 < b1) fine = wait(next);
+        logits(next, scales[1].x, xn);  // formed again below if a new pair begins there; of no use behind the last block
+        fine = fine && wait(DEPTH + slot);
+        const uint32_t vs = base + (uint32_t)((DEPTH + slot) * ring<HD>::HALF);
+        const int left = at.len - at.blk * BLK;
+        if (left < BLK) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if (row_of<HD>(j, 2 * t) >= left) x[j][0] = -INFINITY;
+                if (row_of<HD>(j, 2 * t + 1) >= left) x[j][1] = -INFINITY;
+            }
+        }
+        if (p.scores) {
+            const int head0 = at.inner / p.tiles * p.group + (at.inner % p.tiles) * 8, live = min(8, p.group - (at.inner % p.tiles) * 8);
+            if (g < live) {
+                float* to = p.scores + ((int64_t)at.seq * heads + head0 + g) * c.ctx + at.blk * BLK;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    if (row_of<HD>(j, 2 * t) < left) to[row_of<HD>(j, 2 * t)] = x[j][0];
+                    if (row_of<HD>(j, 2 * t + 1) < left) to[row_of<HD>(j, 2 * t + 1)] = x[j][1];
+                }
+            }
+        }
+        float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1])), fmaxf(fmaxf(x[2][0], x[2][1]), fmaxf(x[3][0], x[3][1])));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float m1 = fmaxf(m, top), use = m1 == -INFINITY ? 0.0f : m1, v_scale = scales[0].y;
+        // the values' scales are taken relative to a power of two above the largest so far, so that their product with a
+        // probability keeps 22 bits in two F16
+        const float vt = __uint_as_float(max(__float_as_uint(v_scale) & 0x7f800000u, 0x0d800000u) + 0x00800000u);  // 2^k > v_scale, at least 2^-99
+        if (__any_sync(0xffffffffu, m1 > m || vt > vtop)) {
+            const float keep = ex2(m - use);
+            const float vt1 = fmaxf(vt, vtop), vinv1 = __uint_as_float((254u << 23) - __float_as_uint(vt1)), keep_o = keep * (vtop * vinv1);
+            l *= keep;
+#pragma unroll
+            for (int i = 0; i < NW * 4; i++) o[i] = f2_mul(o[i], f2_pack(keep_o, keep_o));
+            m = m1, vtop = vt1, vinv = vinv1;
+        }
+        const float vr = v_scale * vinv;
+        // rows of a last block that lie behind the length have probability 0, and whole numbers as values, whatever they are
+        uint32_t ph[4], pl[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float p0 = ex2(x[j][0] - use), p1 = ex2(x[j][1] - use);
+            l += p0 + p1;
+            split2(p0 * vr, p1 * vr, ph[j], pl[j]);
+        }
+        uint32_t r[2][4][NW];  // [half of the block][row][word]
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int row = row_of<HD>(2 * h + (i >> 1), 2 * t + (i & 1));
+                if constexpr (HD == 128) {
+                    const uint4 v = lds128(vs + tile_at<HD>(row, (g >> 1) + 4 * (g & 1)));
+                    r[h][i][0] = v.x ^ 0x80808080u, r[h][i][1] = v.y ^ 0x80808080u, r[h][i][2] = v.z ^ 0x80808080u, r[h][i][3] = v.w ^ 0x80808080u;
+                } else {
+                    const uint2 v = lds64(vs + tile_at<HD>(row, g >> 1) + ((g & 1) << 3));
+                    r[h][i][0] = v.x ^ 0x80808080u, r[h][i][1] = v.y ^ 0x80808080u;
+                }
+            }
+        // The tensor cores cut their sums off instead of rounding them, which over thousands of rows would add up to one
+        // side: a block's sum is formed there and added to the running one by an ordinary addition.
+#pragma unroll
+        for (int n = 0; n < NW; n++) {
+            float y[4][4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) y[j][0] = y[j][1] = y[j][2] = y[j][3] = 0.0f;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {  // 16 rows a step: bytes of two rows side by side, then as pairs of F16
+                const uint32_t a0 = __byte_perm(r[h][0][n], r[h][1][n], 0x5140), a1 = __byte_perm(r[h][0][n], r[h][1][n], 0x7362);
+                const uint32_t c0 = __byte_perm(r[h][2][n], r[h][3][n], 0x5140), c1 = __byte_perm(r[h][2][n], r[h][3][n], 0x7362);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const uint32_t sel = (j & 1) ? 0x4342 : 0x4140;
+                    mma16816(y[j], ph[2 * h], pl[2 * h], ph[2 * h + 1], pl[2 * h + 1], minus_1152(__byte_perm(j < 2 ? a0 : a1, 0x64646464u, sel)),
+                             minus_1152(__byte_perm(j < 2 ? c0 : c1, 0x64646464u, sel)));
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) o[n * 4 + j] = add2(o[n * 4 + j], add2(f2_pack(y[j][0], y[j][1]), f2_pack(y[j][2], y[j][3])));
+        }
+        __syncwarp();
+        if (more) fetch_values(slot);
+#pragma unroll
+        for (int i = 0; i < DEPTH; i++) scales[i] = scales[i + 1];
+        const int64_t item = (int64_t)at.seq * per + at.inner;
+        const int live = min(8, p.group - (at.inner % p.tiles) * 8);
+        at.advance(p.lens, c.seqs, c.ctx, per);
+        slot = next;
+        if (at.blk == 0 || b + 1 == b1) {  // this warp's piece of the pair
+            l += __shfl_xor_sync(0xffffffffu, l, 1);
+            l += __shfl_xor_sync(0xffffffffu, l, 2);
+            if (g < live) {
+                const int64_t row = (w + item) * p.rows + g;
+                if (t == 0) *reinterpret_cast<float2*>(p.stats + 2 * row) = make_float2(m, l);
+                // column 2 t of an n-tile stands for chunk t of a 128-byte row (column 2 t + 1 for chunk t + 4), or bytes 16 t (+ 8) of a 64-byte one
+                float* to = p.acc + row * HD + 16 * t;
+#pragma unroll
+                for (int n = 0; n < NW; n++) {
+                    const uint64_t* on = &o[n * 4];
+                    *reinterpret_cast<float4*>(to + 4 * n) = make_float4(low(on[0]) * vtop, low(on[1]) * vtop, low(on[2]) * vtop, low(on[3]) * vtop);
+                    *reinterpret_cast<float4*>(to + (HD == 128 ? 64 : 8) + 4 * n) = make_float4(high(on[0]) * vtop, high(on[1]) * vtop, high(on[2]) * vtop, high(on[3]) * vtop);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < NW * 4; i++) o[i] = 0;
+            m = -INFINITY, l = 0.0f, vtop = 0.0f, vinv = 0.0f;
+            if (b + 1 < b1) {
+                load_query();
+                logits(next, scales[0].x, xn);
+            }
+        }
+        __syncwarp();
+        more = fetched < b1;
+        if (more) scales[DEPTH] = fetch_keys(next);
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[j][0] = xn[j][0], x[j][1] = xn[j][1];
+    }
+    if (!fine) {  // a copy that does not arrive: reported, and the others are waited for, each with its limit
+        if (lane == 0) *p.status = GALOIS_B200_E_TIMEOUT;
+        for (int i = 0; i < 2 * DEPTH; i++) wait(i);
+    }
+}
+
+// Joins the pieces of one head of one sequence, in their order.  W warps share a head's pieces: one where there are many
+// heads (a head then has a few pieces), eight where there are few and each has up to one from every warp.
+template <int HD, int W>
+__global__ void __launch_bounds__(256) cache_join_kernel(const int32_t* __restrict__ lens, int nseq, int ctx, int kv_heads, int group, int tiles, int rows,
+                                                         int warps, const float* __restrict__ acc, const float* __restrict__ stats,
+                                                         float* __restrict__ out, int64_t o_head, int64_t o_seq, float* __restrict__ final_stats) {
+    gb_pdl_entry();
+    constexpr int E = HD / 32, PER_CTA = 8 / W;
+    __shared__ float part[8][HD];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wr = warp % W;
+    const int heads = kv_heads * group, head = blockIdx.x * PER_CTA + warp / W, s = blockIdx.y;
+    const int per = kv_heads * tiles, inner = head / group * tiles + head % group / 8, r = head % group % 8;
+    const int blocks = (checked_len(lens[s], ctx) + BLK - 1) / BLK;
+    const bool live = head < heads;
+    float* to = out + head * o_head + s * o_seq + lane * E;
+    float l = 0.0f, use = 0.0f, x[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) x[e] = 0.0f;
+    if (live && blocks > 0) {
+        int64_t before = 0, total = 0;  // blocks of the sequences before s, of all
+        for (int i = lane; i < nseq; i += 32) {
+            const int n = (checked_len(lens[i], ctx) + BLK - 1) / BLK;
+            total += n;
+            if (i < s) before += n;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o), before += __shfl_xor_sync(0xffffffffu, before, o);
+        const deal D(total * per, warps);
+        const int64_t first = before * per + (int64_t)inner * blocks;
+        const int w0 = D.owner(first), n = D.owner(first + blocks - 1) - w0 + 1;
+        const int64_t row0 = (w0 + (int64_t)s * per + inner) * rows + r;
+        float m = -INFINITY;
+        for (int i = lane; i < n; i += 32) m = fmaxf(m, stats[2 * (row0 + (int64_t)i * rows)]);
+        m = gb_warp_max(m);
+        use = m == -INFINITY ? 0.0f : m;
+        for (int i = lane; i < n; i += 32) {
+            const float2 st = *reinterpret_cast<const float2*>(stats + 2 * (row0 + (int64_t)i * rows));
+            l += st.y * ex2(st.x - use);
+        }
+        l = gb_warp_sum(l);
+#pragma unroll 4
+        for (int i = wr; i < n; i += W) {
+            const int64_t row = row0 + (int64_t)i * rows;
+            const float f = ex2(stats[2 * row] - use);
+            const float* a = acc + row * HD + lane * E;
+#pragma unroll
+            for (int e = 0; e < E; e++) x[e] = fmaf(a[e], f, x[e]);
+        }
+    }
+    if constexpr (W > 1) {
+#pragma unroll
+        for (int e = 0; e < E; e++) part[warp][lane * E + e] = x[e];
+        __syncthreads();
+        if (wr == 0) {
+#pragma unroll
+            for (int i = 1; i < W; i++)
+#pragma unroll
+                for (int e = 0; e < E; e++) x[e] += part[warp + i][lane * E + e];
+        }
+    }
+    if (live && wr == 0) {
+#pragma unroll
+        for (int e = 0; e < E; e++) to[e] = l == 0.0f ? 0.0f : x[e] / l;
+        if (final_stats && lane == 0) *reinterpret_cast<float2*>(final_stats + 2 * ((int64_t)s * heads + head)) = make_float2(use, l);
     }
 }
 
@@ -62,22 +495,37 @@ __global__ void __launch_bounds__(256) cache_weights_kernel(const int32_t* __res
                                                             int64_t wo_seq, int heads, int kv_heads, int ctx) {
     gb_pdl_entry();
     const int j = blockIdx.x * 256 + threadIdx.x, kh = blockIdx.y, s = blockIdx.z, group = heads / kv_heads;
-    const int n = lens[s];
-    if (n < 0 || n > ctx || j >= n) return;
+    if (j >= checked_len(lens[s], ctx)) return;
     float x = 0.0f;
     for (int g = 0; g < group; g++) {
         const int64_t at = (int64_t)s * heads + kh * group + g;
-        const float m = stats[2 * at], l = stats[2 * at + 1], sc = scores[at * ctx + j];
-        if (sc != -INFINITY) x += expf(sc - m) / l;
+        const float2 ml = *reinterpret_cast<const float2*>(stats + 2 * at);
+        x += ex2(scores[at * ctx + j] - ml.x) / ml.y;
     }
     weights_out[kh * wo_head + s * wo_seq + j] = weights[kh * w_head + s * w_seq + j] + x;
 }
 
-size_t workspace_floats(const gb_cache_view& c, int heads, bool weights) {
-    return 4 + (weights ? (size_t)c.seqs * heads * (2 + (size_t)c.ctx) : 0);
-}
+// Floats of the workspace's parts, each a multiple of 4.
+struct layout {
+    size_t acc, stats, final_stats, scores, total;
+    layout(const galois_b200_ctx* ctx, const gb_cache_view& c, int heads, bool weights) {
+        const int group = c.kv_heads ? heads / c.kv_heads : 0, rows = group < 8 ? group : 8, tiles = (group + 7) / 8;
+        const size_t pieces = (size_t)ctx->sm_count * WARPS + (size_t)c.seqs * c.kv_heads * tiles;
+        acc = 0;
+        stats = acc + pieces * rows * c.head_dim;
+        final_stats = stats + (pieces * rows * 2 + 3) / 4 * 4;
+        scores = final_stats + (weights ? ((size_t)c.seqs * heads * 2 + 3) / 4 * 4 : 0);
+        total = scores + (weights ? (size_t)c.seqs * heads * c.ctx : 0) + 4;
+    }
+};
 
 }  // namespace
+
+int gb_cache_attention_init(galois_b200_ctx* ctx) {
+    GB_CUDA(ctx, cudaFuncSetAttribute(cache_attention_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, ring<64>::TOTAL));
+    GB_CUDA(ctx, cudaFuncSetAttribute(cache_attention_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, ring<128>::TOTAL));
+    return 0;
+}
 
 extern "C" int galois_b200_cache_attention_workspace_bytes(galois_b200_ctx* ctx, const galois_b200_cache_q8* cache, int heads, int with_weights,
                                                            size_t* out_bytes) {
@@ -88,7 +536,7 @@ extern "C" int galois_b200_cache_attention_workspace_bytes(galois_b200_ctx* ctx,
     if (!out_bytes) return gb_fail(ctx, GALOIS_B200_E_BADARG, "cache_attention_workspace_bytes: null pointer");
     if (heads < 0 || (heads && (c.kv_heads == 0 || heads % c.kv_heads)) || heads > 65535)
         return gb_fail(ctx, GALOIS_B200_E_BROADCAST, "cache_attention_workspace_bytes: %d heads over %d key/value heads", heads, c.kv_heads);
-    *out_bytes = workspace_floats(c, heads, with_weights != 0) * sizeof(float);
+    *out_bytes = layout(ctx, c, heads, with_weights != 0).total * sizeof(float);
     return 0;
 }
 
@@ -115,7 +563,7 @@ extern "C" int galois_b200_cache_attention_f32(galois_b200_ctx* ctx, const float
         (c.seqs > 1 && (qd->nb[2] % 4 || dd->nb[2] % 4)) || (uintptr_t)lens % 4 || (uintptr_t)workspace % 16)
         return gb_fail(ctx, GALOIS_B200_E_LAYOUT, "%s: rows of q and dst must be contiguous, they and the workspace 16-byte aligned", what);
     if (!gb_injective(dd)) return gb_fail(ctx, GALOIS_B200_E_DST, "%s: rows of dst overlap", what);
-    const size_t qn = gb_span(qd, 4), dn = gb_span(dd, 4), ln = 4 * (size_t)c.seqs, need = workspace_floats(c, (int)heads, weights != nullptr) * sizeof(float);
+    const size_t qn = gb_span(qd, 4), dn = gb_span(dd, 4), ln = 4 * (size_t)c.seqs, need = layout(ctx, c, (int)heads, weights != nullptr).total * sizeof(float);
     if (workspace_bytes < need) return gb_fail(ctx, GALOIS_B200_E_NOMEM, "%s: workspace of %zu bytes, %zu are needed", what, workspace_bytes, need);
     size_t wn = 0, won = 0;
     if (weights) {
@@ -142,14 +590,31 @@ extern "C" int galois_b200_cache_attention_f32(galois_b200_ctx* ctx, const float
         if (bad) return gb_fail(ctx, GALOIS_B200_E_DST, "%s: dst, workspace or weights_out overlap each other or an operand", what);
     }
     gb_on_device on(ctx);
-    float* stats = weights ? (float*)workspace + 4 : nullptr;
-    float* scores = weights ? stats + 2 * (size_t)c.seqs * heads : nullptr;
-    auto kern = c.head_dim == 64 ? cache_attention_kernel<64> : cache_attention_kernel<128>;
-    GB_CUDA(ctx, gb_launch(ctx, kern, dim3((unsigned)heads, (unsigned)c.seqs), dim3(128), 0, q, qd->nb[1], qd->nb[2], c, lens, dst, dd->nb[1], dd->nb[2],
-                           (int)heads, scale, stats, scores, ctx->dev_status));
-    GB_LAUNCHED(ctx, what);
+    const layout L(ctx, c, (int)heads, weights != nullptr);
+    float* ws = (float*)workspace;
+    float *final_stats = weights ? ws + L.final_stats : nullptr, *scores = weights ? ws + L.scores : nullptr;
+    const int group = (int)heads / c.kv_heads, tiles = (group + 7) / 8, rows = group < 8 ? group : 8;
+    if (c.ctx > 0) {  // else every length is 0
+        CUtensorMap k_map, v_map;
+        const uint64_t size[4] = {(uint64_t)c.head_dim, (uint64_t)c.ctx, (uint64_t)c.kv_heads, (uint64_t)c.seqs};
+        // the stride of a dimension of one element means nothing, but has to be a valid one
+        const uint64_t stride[3] = {c.ctx > 1 ? (uint64_t)c.tok : 128, c.kv_heads > 1 ? (uint64_t)c.head : 128, c.seqs > 1 ? (uint64_t)c.seq : 128};
+        const uint32_t box[4] = {(uint32_t)c.head_dim, BLK, 1, 1};
+        int r = gb_tensor_map(ctx, &k_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, c.k, size, stride, box, c.head_dim);
+        if (r == 0) r = gb_tensor_map(ctx, &v_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, c.v, size, stride, box, c.head_dim);
+        if (r) return r;
+        const step_args a{q, qd->nb[1], qd->nb[2], c, lens, group, tiles, rows, scale, ws + L.acc, ws + L.stats, scores, ctx->dev_status};
+        GB_CUDA(ctx, gb_launch(ctx, c.head_dim == 64 ? cache_attention_kernel<64> : cache_attention_kernel<128>, dim3((unsigned)ctx->sm_count),
+                               dim3(WARPS * 32), c.head_dim == 64 ? ring<64>::TOTAL : ring<128>::TOTAL, a, k_map, v_map));
+        GB_LAUNCHED(ctx, what);
+    }
+    const bool few = (int64_t)heads * c.seqs < 4 * ctx->sm_count;
+    auto join = c.head_dim == 64 ? (few ? cache_join_kernel<64, 8> : cache_join_kernel<64, 1>) : (few ? cache_join_kernel<128, 8> : cache_join_kernel<128, 1>);
+    GB_CUDA(ctx, gb_launch(ctx, join, dim3((unsigned)(few ? heads : (heads + 7) / 8), (unsigned)c.seqs), dim3(256), 0, lens, c.seqs, c.ctx, c.kv_heads, group,
+                           tiles, rows, ctx->sm_count * WARPS, ws + L.acc, ws + L.stats, dst, dd->nb[1], dd->nb[2], final_stats));
+    GB_LAUNCHED(ctx, "cache_join");
     if (weights && c.ctx) {
-        GB_CUDA(ctx, gb_launch(ctx, cache_weights_kernel, dim3((unsigned)((c.ctx + 255) / 256), (unsigned)c.kv_heads, (unsigned)c.seqs), dim3(256), 0, lens, stats,
+        GB_CUDA(ctx, gb_launch(ctx, cache_weights_kernel, dim3((unsigned)((c.ctx + 255) / 256), (unsigned)c.kv_heads, (unsigned)c.seqs), dim3(256), 0, lens, final_stats,
                                scores, weights, wd->nb[1], wd->nb[2], weights_out, wod->nb[1], wod->nb[2], (int)heads, c.kv_heads, c.ctx));
         GB_LAUNCHED(ctx, "cache_weights");
     }

@@ -55,6 +55,8 @@ struct gb_cache_view {
     int64_t s_head, s_seq;      // strides of the scales
     int ctx, kv_heads, seqs, head_dim;
 };
+// Sets the shared-memory limits of the attention kernels on the current device.
+int gb_cache_attention_init(galois_b200_ctx* ctx);
 // 0 and *out filled, or a failure of `what`.
 int gb_check_cache(galois_b200_ctx* ctx, const char* what, const galois_b200_cache_q8* cache, gb_cache_view* out);
 
