@@ -200,6 +200,7 @@ extern "C" int galois_b200_init(int ordinal, void* cu_stream, galois_b200_ctx** 
         if (rc == 0) rc = gb_mm_tc_init(ctx);
         if (rc == 0) rc = gb_decode_init(ctx);
         if (rc == 0) rc = gb_cache_attention_init(ctx);
+        if (rc == 0) rc = gb_prompt_attention_init(ctx);
         if (rc != 0) snprintf(g_init_err, sizeof(g_init_err), "%s", ctx->err);
     }
     if (rc != 0) {

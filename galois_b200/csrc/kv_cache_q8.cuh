@@ -57,6 +57,7 @@ struct gb_cache_view {
 };
 // Sets the shared-memory limits of the attention kernels on the current device.
 int gb_cache_attention_init(galois_b200_ctx* ctx);
+int gb_prompt_attention_init(galois_b200_ctx* ctx);
 // 0 and *out filled, or a failure of `what`.
 int gb_check_cache(galois_b200_ctx* ctx, const char* what, const galois_b200_cache_q8* cache, gb_cache_view* out);
 
