@@ -27,10 +27,6 @@ __device__ __forceinline__ float4 load4<__half>(const __half* p) {
     const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
     return make_float4(a.x, a.y, b.x, b.y);
 }
-__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
-    return (uint32_t)(a & 0xff) | ((uint32_t)(b & 0xff) << 8) | ((uint32_t)(c & 0xff) << 16) | ((uint32_t)d << 24);
-}
-
 // ---------------------------------------------------------------- append
 // A CTA of 128 threads looks at `tile` packed tokens of one head, of the keys (z = 0) or the values (z = 1).  Each
 // token there that is the first new one of its block leads the block: the CTA takes all new rows of that block into
@@ -95,11 +91,9 @@ __global__ void __launch_bounds__(128) cache_append_kernel(const T* __restrict__
             const int row = row0 + i * RPP;
             uint32_t* to = reinterpret_cast<uint32_t*>(out + row * c.tok);
             if (row >= lo && row < hi) {
-                *to = d > 0.0f ? pack4(gb_q8_round(r[i].x, d, rd), gb_q8_round(r[i].y, d, rd), gb_q8_round(r[i].z, d, rd), gb_q8_round(r[i].w, d, rd)) : 0u;
+                *to = d > 0.0f ? gb_q8_round4(r[i], d, rd) : 0u;
             } else if (row < lo && d != held) {
-                const uint32_t w = *to;
-                *to = pack4(gb_q8_rescale(gb_sx(w, 0), held, d, ratio), gb_q8_rescale(gb_sx(w, 1), held, d, ratio),
-                            gb_q8_rescale(gb_sx(w, 2), held, d, ratio), gb_q8_rescale(gb_sx(w, 3), held, d, ratio));
+                *to = gb_q8_rescale4(*to, held, d, ratio);
             }
         }
         t = min(next, end);
@@ -107,54 +101,65 @@ __global__ void __launch_bounds__(128) cache_append_kernel(const T* __restrict__
 }
 
 // ---------------------------------------------------------------- read
-// A CTA of 128 threads gives back 32 packed rows of one head: a lane turns 8 bytes of a row into 8 values.
+// A CTA of 128 threads gives back 32 packed rows of one head: a lane turns 4 bytes of a row into 4 f32, or 8 into 8 F16, so
+// that a warp's stores are whole lines.
 constexpr int READ_ROWS = 32;
 template <typename T, int HD>
 __global__ void __launch_bounds__(128) cache_read_kernel(gb_cache_view c, const int32_t* __restrict__ starts, const int32_t* __restrict__ pos, int nseq,
                                                          int tokens, T* __restrict__ k, int64_t k_head, int64_t k_tok, T* __restrict__ v,
                                                          int64_t v_head, int64_t v_tok, int* __restrict__ status) {
     gb_pdl_entry();
-    constexpr int LPR = HD / 8, RPP = 128 / LPR, N = READ_ROWS / RPP;
-    const int head = blockIdx.y, col = (threadIdx.x % LPR) * 8;
+    constexpr int V = 16 / sizeof(T), W = V / 4, LPR = HD / V, RPP = 128 / LPR, N = READ_ROWS / RPP;
+    const int head = blockIdx.y, col = (threadIdx.x % LPR) * V;
     const int8_t* q = (blockIdx.z ? c.v : c.k) + head * c.head + col;
     const float* scales = (blockIdx.z ? c.vs : c.ks) + head * c.s_head;
     T* y = (blockIdx.z ? v + head * v_head : k + head * k_head) + col;
     const int64_t y_tok = blockIdx.z ? v_tok : k_tok;
+    const int t0 = (int)blockIdx.x * READ_ROWS + threadIdx.x / LPR;
     int s = gb_find_seq(starts, nseq, (int)blockIdx.x * READ_ROWS);
-    uint2 w[N];
+    int begin = 0, end = 0, p0 = 0;
+    if (s < nseq) begin = starts[s], end = starts[s + 1], p0 = pos[s];
+    uint32_t w[N][W];
     float d[N];
-    int row[N];
+    bool live[N];
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        const int t = (int)blockIdx.x * READ_ROWS + threadIdx.x / LPR + i * RPP;
-        row[i] = -1;
-        while (s < nseq && starts[s + 1] <= t) s++;
+        const int t = t0 + i * RPP;
+        live[i] = false;
+        while (s < nseq && end <= t) {
+            if (++s < nseq) begin = end, end = starts[s + 1], p0 = pos[s];
+        }
         if (t < tokens && s < nseq) {
-            const int begin = starts[s], p0 = pos[s];
-            if (begin < 0 || begin > t || starts[s + 1] > tokens || p0 < 0 || p0 >= c.ctx - (t - begin)) {
+            if (begin < 0 || begin > t || end > tokens || p0 < 0 || p0 >= c.ctx - (t - begin)) {
                 *status = GALOIS_B200_E_BADARG;
             } else {
                 const int p = p0 + (t - begin);
-                row[i] = t;
-                w[i] = *reinterpret_cast<const uint2*>(q + s * c.seq + p * c.tok);
+                live[i] = true;
+                const int8_t* from = q + s * c.seq + p * c.tok;
+                if constexpr (W == 1) {
+                    w[i][0] = *reinterpret_cast<const uint32_t*>(from);
+                } else {
+                    const uint2 u = *reinterpret_cast<const uint2*>(from);
+                    w[i][0] = u.x, w[i][1] = u.y;
+                }
                 d[i] = scales[s * c.s_seq + p / GB_CACHE_BLOCK];
             }
         }
     }
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        if (row[i] < 0) continue;
-        float f[8];
+        if (!live[i]) continue;
+        T* to = y + (int64_t)(t0 + i * RPP) * y_tok;
+        float4 f[W];
 #pragma unroll
-        for (int j = 0; j < 8; j++) f[j] = __fmul_rn((float)gb_sx(j < 4 ? w[i].x : w[i].y, j & 3), d[i]);
-        T* to = y + (int64_t)row[i] * y_tok;
-        if constexpr (sizeof(T) == 4) {
-            reinterpret_cast<float4*>(to)[0] = make_float4(f[0], f[1], f[2], f[3]);
-            reinterpret_cast<float4*>(to)[1] = make_float4(f[4], f[5], f[6], f[7]);
+        for (int j = 0; j < W; j++) {
+            f[j] = gb_q8_float4(w[i][j]);
+            f[j] = make_float4(__fmul_rn(f[j].x, d[i]), __fmul_rn(f[j].y, d[i]), __fmul_rn(f[j].z, d[i]), __fmul_rn(f[j].w, d[i]));
+        }
+        if constexpr (W == 1) {
+            *reinterpret_cast<float4*>(to) = f[0];
         } else {
-            __half2 h[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) h[j] = __floats2half2_rn(f[2 * j], f[2 * j + 1]);
+            __half2 h[4] = {__floats2half2_rn(f[0].x, f[0].y), __floats2half2_rn(f[0].z, f[0].w), __floats2half2_rn(f[W - 1].x, f[W - 1].y), __floats2half2_rn(f[W - 1].z, f[W - 1].w)};
             *reinterpret_cast<uint4*>(to) = *reinterpret_cast<uint4*>(h);
         }
     }
@@ -172,37 +177,50 @@ __device__ __forceinline__ uint32_t order_key(float w) {
     const uint32_t k = (u & 0x80000000u) ? ~u : u | 0x80000000u;
     return w == 0.0f ? 0x80000000u : k;  // -0 and 0 are equal
 }
-// Inclusive sum over the CTA's threads; *total receives the sum of all.  `part`: 33 words of shared memory.
-__device__ __forceinline__ int cta_scan(int x, int* part, int* total) {
+// Inclusive sum over the CTA's threads; *total receives the sum of all.  `part`: 32 words of shared memory that are free
+// again after the caller's next __syncthreads.
+__device__ __forceinline__ uint32_t cta_scan(uint32_t x, uint32_t* part, uint32_t* total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
     }
     if (lane == 31) part[warp] = x;
     __syncthreads();
-    if (warp == 0) {
-        int y = part[lane];
+    uint32_t y = part[lane];  // every warp sums the warps' sums
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int z = __shfl_up_sync(0xffffffffu, y, o);
-            if (lane >= o) y += z;
-        }
-        part[lane] = y;
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t z = __shfl_up_sync(0xffffffffu, y, o);
+        if (lane >= o) y += z;
     }
-    __syncthreads();
-    *total = part[31];
-    if (warp > 0) x += part[warp - 1];
-    __syncthreads();
-    return x;
+    *total = __shfl_sync(0xffffffffu, y, 31);
+    const uint32_t in_front = __shfl_sync(0xffffffffu, y, (warp + 31) & 31);
+    return warp ? x + in_front : x;
+}
+// A thread holds EV_EACH consecutive weights of a chunk, so that one sum over the CTA orders the whole chunk; a row of up to
+// 8192 tokens is one chunk and is read once.
+constexpr int EV_EACH = 8, EV_CHUNK = EV_THREADS * EV_EACH;
+__device__ __forceinline__ void load_keys(const float* __restrict__ w, int i0, int n, float (&x)[EV_EACH], uint32_t (&key)[EV_EACH]) {
+    if (i0 + EV_EACH <= n && (uintptr_t)(w + i0) % 16 == 0) {
+        const float4 a = *reinterpret_cast<const float4*>(w + i0), b = *reinterpret_cast<const float4*>(w + i0 + 4);
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    } else {
+#pragma unroll
+        for (int e = 0; e < EV_EACH; e++) x[e] = i0 + e < n ? w[i0 + e] : 0.0f;
+    }
+#pragma unroll
+    for (int e = 0; e < EV_EACH; e++) key[e] = order_key(x[e]);
 }
 __global__ void __launch_bounds__(EV_THREADS) cache_select_kernel(const int32_t* __restrict__ lens, const float* __restrict__ weights, int64_t w_head,
                                                                   int64_t w_seq, int ctx, int budget, int recent, int32_t* __restrict__ out_lens,
                                                                   float* __restrict__ out_weights, int64_t ow_head, int64_t ow_seq,
                                                                   int32_t* __restrict__ index, int64_t i_head, int64_t i_seq, int* __restrict__ status) {
     gb_pdl_entry();
-    __shared__ int hist[256], part[33], pick[2];
+    // the weights of a row lie close together, most of them in a few digits: eight counts of each, dealt by warp
+    __shared__ int hist[8][256];
+    __shared__ uint32_t part[32];
+    __shared__ int pick[2];
     const int head = blockIdx.x, s = blockIdx.y, tid = threadIdx.x;
     int n = lens[s];
     if (n < 0 || n > ctx) {
@@ -214,57 +232,70 @@ __global__ void __launch_bounds__(EV_THREADS) cache_select_kernel(const int32_t*
     int32_t* idx = index + head * i_head + s * i_seq;
     const int m = min(n, budget), r = min(recent, m), cand = n - r, need = m - r;
     if (head == 0 && tid == 0) out_lens[s] = m;
+    float x[EV_EACH];
+    uint32_t key[EV_EACH];
+    const bool once = n <= EV_CHUNK, choose = need > 0 && need < cand;
+    if (once) load_keys(w, tid * EV_EACH, n, x, key);
     // the need-th largest key among the first `cand`: `limit`, and how many of those equal to it are kept
     uint32_t limit = 0;
     int left = need;
-    if (need > 0 && need < cand) {
+    if (choose) {
         uint32_t mask = 0;
         for (int shift = 24; shift >= 0; shift -= 8) {
-            if (tid < 256) hist[tid] = 0;
+            for (int i = tid; i < 8 * 256; i += EV_THREADS) (&hist[0][0])[i] = 0;
             __syncthreads();
-            for (int i = tid; i < cand; i += EV_THREADS) {
-                const uint32_t key = order_key(w[i]);
-                if ((key & mask) == limit) atomicAdd(&hist[(key >> shift) & 255u], 1);
+            for (int c0 = 0; c0 < cand; c0 += EV_CHUNK) {
+                const int i0 = c0 + tid * EV_EACH;
+                if (!once) load_keys(w, i0, n, x, key);
+#pragma unroll
+                for (int e = 0; e < EV_EACH; e++)
+                    if (i0 + e < cand && (key[e] & mask) == limit) atomicAdd(&hist[(tid >> 5) & 7][(key[e] >> shift) & 255u], 1);
             }
             __syncthreads();
             // thread t looks at digit 255 - t: the first whose count of keys at or above reaches `left`
-            int total;
-            const int c = tid < 256 ? hist[255 - tid] : 0;
-            const int upto = cta_scan(c, part, &total);
+            uint32_t total;
+            int c = 0;
+            if (tid < 256) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) c += hist[i][255 - tid];
+            }
+            const int upto = (int)cta_scan((uint32_t)c, part, &total);
             if (tid < 256 && upto >= left && upto - c < left) pick[0] = 255 - tid, pick[1] = left - (upto - c);
             __syncthreads();
             limit |= (uint32_t)pick[0] << shift;
             left = pick[1];
             mask |= 255u << shift;
-            __syncthreads();
         }
     }
-    // rows of the kept tokens, in order
-    int rows = 0, same = 0;
-    for (int i0 = 0; i0 < n; i0 += EV_THREADS) {
-        const int i = i0 + tid;
-        bool above = false, equal = false;
-        float wi = 0.0f;
-        if (i < n) {
-            wi = w[i];
-            if (i >= cand || need >= cand) {
-                above = true;
-            } else if (need > 0) {
-                const uint32_t key = order_key(wi);
-                above = key > limit, equal = key == limit;
+    // rows of the kept tokens, in order: in front of a token are all above the limit and, of those equal to it, `left` at most
+    int above_front = 0, equal_front = 0;
+    for (int c0 = 0; c0 < n; c0 += EV_CHUNK) {
+        const int i0 = c0 + tid * EV_EACH;
+        if (!once) load_keys(w, i0, n, x, key);
+        uint32_t above = 0, equal = 0;  // bit e: token i0 + e
+#pragma unroll
+        for (int e = 0; e < EV_EACH; e++) {
+            const int i = i0 + e;
+            if (i >= n) continue;
+            if (i >= cand || (need > 0 && !choose) || (choose && key[e] > limit)) above |= 1u << e;
+            else if (choose && key[e] == limit) equal |= 1u << e;
+        }
+        uint32_t total;
+        const uint32_t mine = (uint32_t)__popc(above) | ((uint32_t)__popc(equal) << 16);  // both sums are below 2^14
+        const uint32_t front = cta_scan(mine, part, &total) - mine;
+        int a = above_front + (int)(front & 0xffffu), q = equal_front + (int)(front >> 16);
+#pragma unroll
+        for (int e = 0; e < EV_EACH; e++) {
+            const bool is = (above >> e) & 1, tie = (equal >> e) & 1;
+            if (is || (tie && q < left)) {
+                const int at = a + min(q, left);
+                idx[at] = i0 + e;
+                ow[at] = x[e];
             }
+            a += is, q += tie;
         }
-        int total;
-        const int e = cta_scan(equal, part, &total);
-        if (equal && same + e <= left) above = true;
-        same += total;
-        const int k = cta_scan(above, part, &total);
-        if (above) {
-            const int at = rows + k - 1;
-            idx[at] = i;
-            ow[at] = wi;
-        }
-        rows += total;
+        above_front += (int)(total & 0xffffu), equal_front += (int)(total >> 16);
+        __syncthreads();
     }
 }
 
@@ -301,10 +332,7 @@ __global__ void __launch_bounds__(128) cache_gather_kernel(gb_cache_view c, gb_c
         if (d0 != d) {
             uint32_t* p = reinterpret_cast<uint32_t*>(&w);
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                p[j] = d > 0.0f ? pack4(gb_q8_rescale(gb_sx(p[j], 0), d0, d, r), gb_q8_rescale(gb_sx(p[j], 1), d0, d, r),
-                                        gb_q8_rescale(gb_sx(p[j], 2), d0, d, r), gb_q8_rescale(gb_sx(p[j], 3), d0, d, r))
-                                : 0u;
+            for (int j = 0; j < 4; j++) p[j] = d > 0.0f ? gb_q8_rescale4(p[j], d0, d, r) : 0u;
         }
         *reinterpret_cast<uint4*>(out + row * o.tok + col) = w;
     }

@@ -8,20 +8,22 @@
 // 4 head_dim flops a pair of query and key against 4 bytes a token: bound by the tensor cores, and next to them by the
 // exponentials (16 a cycle and SM against 32 pairs a cycle that the tensor cores get through).
 //
-//   warps 0-3, 4-7  soft-max of query tile 0, 1 (128 rows each, a thread per row)
-//   warp 8          loader: TMA copies of the query tiles, then keys and values, 128 rows at a time, through four slots
-//   warp 9          issues the tensor-core products and owns the tensor memory
-//   warp 10         (of 10, 11) looks at the values of tiles that some query does not see whole
+//   warps 0-7, 8-15  soft-max of query tile 0, 1 (128 rows each, two threads per row: 64 logits each)
+//   warp 16          loader: TMA copies of the query tiles, then keys and values, 128 rows at a time, through a ring of slots
+//   warp 17          issues the tensor-core products and owns the tensor memory
+//   warp 18          clears what lies behind a sequence's end in its last tile of values
 //
-// The two query tiles of a CTA share the keys: two heads of a group over the same tokens where the group is even (their
-// masks agree), else two runs of tokens of one head.  While one tile's logits are in the soft-max, the tensor cores work
-// for the other.  Tensor memory: logits 2 x 128 columns, results 2 x head_dim; the probabilities (F16) overwrite the first
-// half of their logits and are the second product's operand from there.  The running maximum that probabilities refer to is
-// raised only when a row's maximum passes it by 2^8 (F16 holds what that leaves), so that the results in tensor memory
-// are rarely rescaled; the logits' barrier also says that the products before them are done, so the rescaling needs no other.
+// One CTA per SM goes through units of two query tiles (those that see most keys first), and every role runs ahead on its
+// own: keys of the next unit are loaded, and its first logits formed, while the results of this one are written.  The two
+// query tiles share the keys: two heads of a group over the same tokens where the group is even (their masks agree), else
+// two runs of tokens of one head.  While one tile's logits are in the soft-max, the tensor cores work for the other.  Tensor
+// memory: logits 2 x 128 columns, results 2 x head_dim; the probabilities (F16) overwrite the first half of their logits and
+// are the second product's operand from there.  The running maximum that probabilities refer to is raised only when a row's
+// maximum passes it by 2^8 (F16 holds what that leaves), so that the results in tensor memory are rarely rescaled; the
+// logits' barrier also says that the products before them are done, so the rescaling needs no other.
 //
-// A probability of 0 does not hide a value that is not finite.  So warp 10 clears the values behind a sequence's end
-// and, should the last tiles hold any number that is not finite, has the CTA's rows formed again by the plain loop below.
+// A probability of 0 does not hide a value that is not finite: where a result is not finite, its rows are formed again by
+// the plain loop below, which reads nothing that a query does not see.
 #include "kv_cache_q8.cuh"
 
 #include "tcgen05.cuh"
@@ -36,42 +38,46 @@ struct rows16 {  // an F16 {head_dim, heads, tokens} operand
     int64_t head, tok;
 };
 
-// One query row by one warp: a lane holds HD / 32 numbers.
+// Half of one query row's result by one warp: a lane holds HD / 32 numbers of the query, HD / 64 of the result.
 template <int HD, typename T>
-__device__ __forceinline__ void prompt_row(const rows16& q, const rows16& k, const rows16& v, int t, int k0, int n, int h, int kh, float scale, T* out) {
-    constexpr int E = HD / 32;
-    const int lane = threadIdx.x & 31;
-    float qr[E], o[E], m = -INFINITY, l = 0.0f;
+__device__ __noinline__ void prompt_row(const rows16& q, const rows16& k, const rows16& v, int t, int k0, int n, int h, int kh, float scale, int half, T* out) {
+    constexpr int E = HD / 32, EO = HD / 64;
+    const int lane = threadIdx.x & 31, col = half * (HD / 2) + lane * EO;
+    float qr[E], o[EO], m = -INFINITY, l = 0.0f;
 #pragma unroll
-    for (int e = 0; e < E; e++) qr[e] = __half2float(q.p[h * q.head + t * q.tok + lane * E + e]) * scale, o[e] = 0.0f;
+    for (int e = 0; e < E; e++) qr[e] = __half2float(q.p[h * q.head + t * q.tok + lane * E + e]) * scale;
+#pragma unroll
+    for (int e = 0; e < EO; e++) o[e] = 0.0f;
     for (int j = 0; j < n; j++) {
         const __half* kr = k.p + kh * k.head + (int64_t)(k0 + j) * k.tok + lane * E;
-        const __half* vr = v.p + kh * v.head + (int64_t)(k0 + j) * v.tok + lane * E;
+        const __half* vr = v.p + kh * v.head + (int64_t)(k0 + j) * v.tok + col;
         float x = 0.0f;
 #pragma unroll
         for (int e = 0; e < E; e++) x = fmaf(qr[e], __half2float(kr[e]), x);
         x = gb_warp_sum(x);
-        const float top = fmaxf(m, x), keep = m == -INFINITY ? 0.0f : expf(m - top), p = x == -INFINITY ? 0.0f : expf(x - top);
+        const float top = x > m || x != x ? x : m, keep = m == -INFINITY ? 0.0f : expf(m - top), p = x == -INFINITY ? 0.0f : expf(x - top);
         m = top;
         l = l * keep + p;
 #pragma unroll
-        for (int e = 0; e < E; e++) o[e] = fmaf(p, __half2float(vr[e]), o[e] * keep);
+        for (int e = 0; e < EO; e++) o[e] = fmaf(p, __half2float(vr[e]), o[e] * keep);
     }
 #pragma unroll
-    for (int e = 0; e < E; e++) {
+    for (int e = 0; e < EO; e++) {
         const float x = l == 0.0f ? 0.0f : o[e] / l;
-        if constexpr (sizeof(T) == 4) out[lane * E + e] = x;
-        else out[lane * E + e] = __float2half_rn(x);
+        if constexpr (sizeof(T) == 4) out[col + e] = x;
+        else out[col + e] = __float2half_rn(x);
     }
 }
 
 constexpr int PT = 128;      // rows of a tile of queries, of keys, of values
-constexpr int SLOTS = 4;     // tiles of keys and values in shared memory
-constexpr int THREADS = 11 * 32;
+constexpr int LOADER = 16, ISSUER = 17, CHECKER = 18;  // warps behind the soft-max's
+constexpr int THREADS = 19 * 32;
 template <int HD>
 struct plan {
     static constexpr uint32_t TILE = PT * HD * 2, HALF = PT * 128;  // bytes of a tile; of its first 64 columns
-    static constexpr uint32_t Q = 0, KV = 2 * TILE, BARS = KV + SLOTS * TILE, TOTAL = 1024 + BARS + 256;
+    static constexpr int SLOTS = HD == 128 ? 5 : 12;                // tiles of keys and values in shared memory
+    static constexpr uint32_t Q = 0, KV = 2 * TILE, BARS = KV + SLOTS * TILE, PAIR = BARS + 320, TOTAL = PAIR + 2 * 2 * PT * 4;
+    static_assert(TOTAL <= 227 * 1024, "shared memory");
 };
 struct prompt_args {
     rows16 q, k, v;
@@ -88,9 +94,10 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// The largest, or NaN if one of them is: a logit that is not a number has to reach the result.
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
 __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
@@ -110,27 +117,81 @@ __device__ __forceinline__ bool sequence(const prompt_args& p, int s, int& q0, i
     return ok;
 }
 
+// Where the CTA's units lie.  Units are counted with the heads fastest and, within a sequence, the tiles that see most keys
+// first.  A warp keeps 32 sequences, a lane each, and goes forward.
+struct unit_finder {
+    int s0, before, mine, upto, q0, nq, k0, nk;  // first sequence held, tiles before it; this lane's sequence
+    __device__ __forceinline__ void load(const prompt_args& p, int span) {
+        const int s = s0 + (threadIdx.x & 31);
+        q0 = nq = k0 = nk = 0;
+        if (s < p.nseq) sequence(p, s, q0, nq, k0, nk);
+        mine = upto = (nq + span - 1) / span;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, upto, o);
+            if ((int)(threadIdx.x & 31) >= o) upto += y;
+        }
+    }
+    __device__ __forceinline__ void start(const prompt_args& p, int span) {
+        s0 = before = 0;
+        load(p, span);
+    }
+};
+// The CTA's unit of a round: forwards, then backwards, so that who had one of the larger units gets one of the smaller.
+__device__ __forceinline__ int64_t unit_of_round(int r) { return (int64_t)r * gridDim.x + ((r & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x); }
+struct prompt_unit {
+    int first, q0, nq, k0, nk;  // the first query's place within the sequence; the sequence
+    int head0, kh;
+    int tiles0, tiles1, n;      // key tiles of the two query tiles, the larger
+    // unit `u` of this launch, or false behind the last
+    __device__ __forceinline__ bool find(const prompt_args& p, unit_finder& f, int64_t u, int units, int span, bool two_heads) {
+        const int unit = (int)(u % units), want = (int)(u / units);
+        uint32_t past;
+        while ((past = __ballot_sync(0xffffffffu, f.before + f.upto > want)) == 0) {
+            if (f.s0 + 32 >= p.nseq) return false;
+            f.before += __shfl_sync(0xffffffffu, f.upto, 31);
+            f.s0 += 32;
+            f.load(p, span);
+        }
+        const int l = __ffs(past) - 1;
+        first = (f.before + __shfl_sync(0xffffffffu, f.upto, l) - 1 - want) * span;
+        q0 = __shfl_sync(0xffffffffu, f.q0, l), nq = __shfl_sync(0xffffffffu, f.nq, l);
+        k0 = __shfl_sync(0xffffffffu, f.k0, l), nk = __shfl_sync(0xffffffffu, f.nk, l);
+        head0 = two_heads ? 2 * unit : unit;
+        kh = head0 / p.group;
+        tiles0 = tiles(0);
+        tiles1 = two_heads ? tiles0 : tiles(PT);
+        n = max(tiles0, tiles1);
+        return true;
+    }
+    __device__ __forceinline__ int tiles(int off) const {
+        const int rows = min(PT, nq - first - off);
+        return rows > 0 ? (max(0, first + off + rows + nk - nq) + PT - 1) / PT : 0;
+    }
+    // the last tile of values reaches behind the sequence's end
+    __device__ __forceinline__ bool ragged() const { return n > 0 && n * PT > nk; }
+};
+
 template <int HD, typename T>
 __global__ void __launch_bounds__(THREADS, 1)
     prompt_attention_kernel(const prompt_args p, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                             const __grid_constant__ CUtensorMap v_map) {
     using L = plan<HD>;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    constexpr int SLOTS = L::SLOTS;
+    extern __shared__ __align__(1024) uint8_t smem[];  // swizzled tiles start at multiples of 1024
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
-    uint64_t *q_full = bars, *full = bars + 1, *empty = full + SLOTS, *s_full = empty + SLOTS, *p_ready = s_full + 2, *o_done = p_ready + 2, *v_raw = o_done + 2;
-    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(v_raw + 2);
-    volatile int* odd = reinterpret_cast<int*>(tmem_at + 1);  // a value that is not finite was seen
+    uint64_t *q_full = bars, *q_free = bars + 1, *full = bars + 2, *empty = full + SLOTS, *s_full = empty + SLOTS, *p_ready = s_full + 2, *o_done = p_ready + 2,
+             *v_raw = o_done + 2;
+    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(v_raw + 1);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) {
         tma_prefetch_map(&q_map), tma_prefetch_map(&k_map), tma_prefetch_map(&v_map);
-        mbar_init(q_full, 1);
+        mbar_init(q_full, 1), mbar_init(q_free, 1), mbar_init(v_raw, 1);
         for (int i = 0; i < SLOTS; i++) mbar_init(full + i, 1), mbar_init(empty + i, 1);
-        for (int i = 0; i < 2; i++) mbar_init(s_full + i, 1), mbar_init(p_ready + i, 4), mbar_init(o_done + i, 1), mbar_init(v_raw + i, 1);
+        for (int i = 0; i < 2; i++) mbar_init(s_full + i, 1), mbar_init(p_ready + i, 8), mbar_init(o_done + i, 1);
         fence_mbarrier_init_cluster();
-        *odd = 0;
     }
-    if (warp == 9) {
+    if (warp == ISSUER) {
         tc_alloc(tmem_at, 512);
         tc_relinquish();
     }
@@ -140,245 +201,258 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t tmem = *tmem_at;
     gb_pdl_entry();
 
-    // ---- the CTA's queries: heads vary fastest, and the last tokens of a sequence, which see the most keys, come first
     const bool two_heads = p.group % 2 == 0;
     const int units = two_heads ? p.heads / 2 : p.heads, span = two_heads ? PT : 2 * PT;
-    const int unit = (int)(blockIdx.x % (unsigned)units), want = (int)(blockIdx.x / (unsigned)units);
-    int seq = -1, tile = 0, q0 = 0, nq = 0, k0 = 0, nk = 0;
-    for (int s0 = 0, before = 0; s0 < p.nseq; s0 += 32) {
-        int a, n = 0, c, d;
-        if (s0 + lane < p.nseq && !sequence(p, s0 + lane, a, n, c, d) && blockIdx.x == 0 && warp == 0) *p.status = GALOIS_B200_E_BADARG;
-        const int mine = (n + span - 1) / span;
-        int upto = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += y;
-        }
-        const uint32_t past = __ballot_sync(0xffffffffu, before + upto > want);
-        if (past && seq < 0) {
-            const int l = __ffs(past) - 1, tiles = __shfl_sync(0xffffffffu, mine, l);
-            seq = s0 + l;
-            tile = tiles - 1 - (want - before - (__shfl_sync(0xffffffffu, upto, l) - tiles));
-            if (blockIdx.x != 0) break;  // the first CTA looks at all starts
-        }
-        before += __shfl_sync(0xffffffffu, upto, 31);
-    }
-    if (seq >= 0) sequence(p, seq, q0, nq, k0, nk);
-    // per query tile s: its first token (within the sequence), its head, its valid rows, its key tiles
-    const int head0 = two_heads ? 2 * unit : unit, kh = head0 / p.group;
-    int n_tiles[2];
-#pragma unroll
-    for (int s = 0; s < 2; s++) {
-        const int first = tile * span + (two_heads ? 0 : s * PT), rows = seq < 0 ? 0 : max(0, min(PT, nq - first));
-        n_tiles[s] = rows > 0 ? (max(0, first + rows + nk - nq) + PT - 1) / PT : 0;
-    }
-    const int n = max(n_tiles[0], n_tiles[1]);
-    const int whole = max(0, tile * span + nk - nq + 1) / PT;  // key tiles that every query sees whole
+    unit_finder f;
+    if (warp >= LOADER) f.start(p, span);
+    prompt_unit x;
     bool fine = true;
 
-    if (warp == 8) {
-        if (lane == 0 && n > 0) {
-            mbar_expect_tx(q_full, 2 * L::TILE);
-            for (int s = 0; s < 2; s++)
-                for (int h = 0; h < HD / 64; h++)
-                    tma_load_3d(smem_u32(smem + L::Q) + s * L::TILE + h * L::HALF, &q_map, 64 * h, q0 + tile * span + (two_heads ? 0 : s * PT),
-                                two_heads ? head0 + s : head0, q_full);
-            int i = 0;
-            for (; i < 2 * n; i++) {
-                const int slot = i % SLOTS;
-                if (i >= SLOTS && !mbar_wait_bounded(empty + slot, (i / SLOTS - 1) & 1)) {
-                    fine = false;
-                    break;
-                }
-                // values that warp 10 looks at arrive at a barrier of its own; it passes them on
-                uint64_t* bar = (i & 1) && (i >> 1) >= whole ? v_raw + (((i >> 1) - whole) & 1) : full + slot;
-                mbar_expect_tx(bar, L::TILE);
-                for (int h = 0; h < HD / 64; h++)
-                    tma_load_3d(smem_u32(smem + L::KV) + slot * L::TILE + h * L::HALF, (i & 1) ? &v_map : &k_map, 64 * h, k0 + (i >> 1) * PT, kh, bar);
-            }
-            if (!fine) {  // leave no copy of its own in flight
-                mbar_wait_bounded(q_full, 0);
-                for (int j = max(0, i - SLOTS); j < i; j++) mbar_wait_bounded(full + j % SLOTS, (j / SLOTS) & 1);
-            }
-        }
-        __syncwarp();
-    } else if (warp == 9) {
-        if (lane == 0 && n > 0) {
-            // f32 sums, F16 operands; logits: keys as they are; results: values with the contraction along their rows
-            const uint32_t idesc_s = (1u << 4) | ((uint32_t)(PT >> 3) << 17) | ((uint32_t)(PT >> 4) << 24);
-            const uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(PT >> 4) << 24);
-            const uint32_t q_at = smem_u32(smem + L::Q), kv_at = smem_u32(smem + L::KV);
-            auto logits = [&](int s, int j) {
-                const uint32_t k_at = kv_at + (uint32_t)((2 * j) % SLOTS) * L::TILE;
-#pragma unroll
-                for (int kk = 0; kk < HD / 16; kk++) {
-                    const uint32_t off = (kk / 4) * L::HALF + (kk % 4) * 32;
-                    tc_mma_f16_ss(tmem + s * PT, tc_desc(q_at + s * L::TILE + off, 16, 1024, 128), tc_desc(k_at + off, 16, 1024, 128), idesc_s, kk > 0);
-                }
-                tc_commit(s_full + s);
-            };
-            fine = mbar_wait_bounded(q_full, 0) && mbar_wait_bounded(full, 0);
-            if (fine) {
-                for (int s = 0; s < 2; s++)
-                    if (n_tiles[s] > 0) logits(s, 0);
-                tc_commit(empty);
-            }
-            for (int j = 0; j < n && fine; j++) {
-                const int vs = (2 * j + 1) % SLOTS, ks = (2 * j + 2) % SLOTS;
-                fine = mbar_wait_bounded(full + vs, ((2 * j + 1) / SLOTS) & 1) && (j + 1 >= n || mbar_wait_bounded(full + ks, ((2 * j + 2) / SLOTS) & 1));
-                for (int s = 0; s < 2 && fine; s++) {
-                    if (j >= n_tiles[s]) continue;
-                    fine = mbar_wait_bounded(p_ready + s, j & 1);
-                    if (!fine) break;
-                    tc_after_sync();
-#pragma unroll
-                    for (int kk = 0; kk < PT / 16; kk++)
-                        tc_mma_f16_ts(tmem + 2 * PT + s * HD, tmem + s * PT + kk * 8, tc_desc(kv_at + vs * L::TILE + kk * 2048, L::HALF, 1024, 128), idesc_o, j > 0 || kk > 0);
-                    if (j + 1 < n_tiles[s]) logits(s, j + 1);
-                    else tc_commit(o_done + s);
-                }
+    if (warp == LOADER) {
+        int it = 0, nu = 0;  // tiles of keys and values so far, units with any
+        for (int r = 0; fine && x.find(p, f, unit_of_round(r), units, span, two_heads); r++) {
+            if (x.n == 0) continue;
+            if (lane == 0) {
+                if (nu > 0) fine = mbar_try_bounded(q_free, (nu - 1) & 1);
                 if (fine) {
-                    tc_commit(empty + vs);
-                    if (j + 1 < n) tc_commit(empty + ks);
+                    mbar_expect_tx(q_full, 2 * L::TILE);
+                    for (int s = 0; s < 2; s++)
+                        for (int h = 0; h < HD / 64; h++)
+                            tma_load_3d(smem_u32(smem + L::Q) + s * L::TILE + h * L::HALF, &q_map, 64 * h, x.q0 + x.first + (two_heads ? 0 : s * PT),
+                                        two_heads ? x.head0 + s : x.head0, q_full);
+                }
+                for (int i = 0; i < 2 * x.n && fine; i++, it++) {
+                    const int slot = it % SLOTS;
+                    if (it >= SLOTS) fine = mbar_try_bounded(empty + slot, (it / SLOTS - 1) & 1);
+                    if (!fine) break;
+                    // a last tile of values that warp 18 has to clear arrives at a barrier of its own; it passes the tile on
+                    uint64_t* bar = i == 2 * x.n - 1 && x.ragged() ? v_raw : full + slot;
+                    mbar_expect_tx(bar, L::TILE);
+                    for (int h = 0; h < HD / 64; h++)
+                        tma_load_3d(smem_u32(smem + L::KV) + slot * L::TILE + h * L::HALF, (i & 1) ? &v_map : &k_map, 64 * h, x.k0 + (i >> 1) * PT, x.kh, bar);
                 }
             }
+            nu++;
+            fine = __shfl_sync(0xffffffffu, (int)fine, 0);
         }
-        __syncwarp();
-    } else if (warp == 10) {
-        for (int j = whole; j < n && fine; j++) {
-            const int slot = (2 * j + 1) % SLOTS, valid = min(PT, nk - j * PT);
-            fine = __all_sync(0xffffffffu, mbar_wait_bounded(v_raw + ((j - whole) & 1), ((j - whole) >> 1) & 1));
-            if (!fine) break;
-            uint4* v = reinterpret_cast<uint4*>(smem + L::KV + slot * L::TILE);  // [half][row][8 pieces]
-            uint32_t bad = 0;
-#pragma unroll 8
-            for (int x = lane; x < (int)L::TILE / 16; x += 32) {
-                if ((x >> 3) % PT < valid) {
-                    const uint4 w = v[x];
-                    // an exponent of all ones carries into the sign's place
-                    bad |= ((w.x & 0x7c007c00u) + 0x04000400u) | ((w.y & 0x7c007c00u) + 0x04000400u) | ((w.z & 0x7c007c00u) + 0x04000400u) |
-                           ((w.w & 0x7c007c00u) + 0x04000400u);
-                } else {
-                    v[x] = make_uint4(0, 0, 0, 0);
+        // no arrival and no copy is left under way: the last tiles have been used (or, after a time-out, have had time to land)
+        if (lane == 0) {
+            for (int i = max(0, it - SLOTS); i < it; i++) {
+                if (fine) fine = mbar_try_bounded(empty + i % SLOTS, (i / SLOTS) & 1);
+                else mbar_try_bounded(full + i % SLOTS, (i / SLOTS) & 1);
+            }
+            if (fine && nu > 0) fine = mbar_try_bounded(q_free, (nu - 1) & 1);
+        }
+    } else if (warp == ISSUER) {
+        // f32 sums, F16 operands; logits: keys as they are; results: values with the contraction along their rows
+        const uint32_t idesc_s = (1u << 4) | ((uint32_t)(PT >> 3) << 17) | ((uint32_t)(PT >> 4) << 24);
+        const uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(PT >> 4) << 24);
+        const uint32_t q_at = smem_u32(smem + L::Q), kv_at = smem_u32(smem + L::KV);
+        int it = 0, nu = 0;
+        int ready[2] = {0, 0};  // tiles of each query tile whose probabilities have been waited for
+        auto logits = [&](int s, int slot) {
+            const uint32_t k_at = kv_at + (uint32_t)slot * L::TILE;
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; kk++) {
+                const uint32_t off = (kk / 4) * L::HALF + (kk % 4) * 32;
+                tc_mma_f16_ss(tmem + s * PT, tc_desc(q_at + s * L::TILE + off, 16, 1024, 128), tc_desc(k_at + off, 16, 1024, 128), idesc_s, kk > 0);
+            }
+            tc_commit(s_full + s);
+        };
+        for (int r = 0; fine && x.find(p, f, unit_of_round(r), units, span, two_heads); r++) {
+            if (x.n == 0) continue;
+            if (lane == 0) {
+                const int tiles[2] = {x.tiles0, x.tiles1};
+                fine = mbar_try_bounded(q_full, nu & 1) && mbar_try_bounded(full + it % SLOTS, (it / SLOTS) & 1);
+                if (fine) {
+                    for (int s = 0; s < 2; s++)
+                        if (tiles[s] > 0) logits(s, it % SLOTS);
+                    tc_commit(empty + it % SLOTS);
+                    if (x.n == 1) tc_commit(q_free);
+                }
+                for (int j = 0; j < x.n && fine; j++) {
+                    const int vi = it + 2 * j + 1, vs = vi % SLOTS, ki = vi + 1, ks = ki % SLOTS;
+                    fine = mbar_try_bounded(full + vs, (vi / SLOTS) & 1);
+                    bool keys = false;  // the next keys have arrived
+                    for (int s = 0; s < 2 && fine; s++) {
+                        if (j >= tiles[s]) continue;
+                        fine = mbar_try_bounded(p_ready + s, ready[s] & 1);
+                        ready[s]++;
+                        if (!fine) break;
+                        tc_after_sync();
+#pragma unroll
+                        for (int kk = 0; kk < PT / 16; kk++)
+                            tc_mma_f16_ts(tmem + 2 * PT + s * HD, tmem + s * PT + kk * 8, tc_desc(kv_at + vs * L::TILE + kk * 2048, L::HALF, 1024, 128), idesc_o, j > 0 || kk > 0);
+                        if (s == 1 || j >= tiles[1]) tc_commit(empty + vs);
+                        if (j + 1 < tiles[s]) {
+                            if (!keys) fine = mbar_try_bounded(full + ks, (ki / SLOTS) & 1);
+                            if (!fine) break;
+                            keys = true;
+                            logits(s, ks);
+                        } else {
+                            tc_commit(o_done + s);
+                        }
+                    }
+                    if (fine && j + 1 < x.n) tc_commit(empty + ks);
+                    if (fine && j + 2 == x.n) tc_commit(q_free);  // the queries have been used for the last time
                 }
             }
-            if (__any_sync(0xffffffffu, (bad & 0x80008000u) != 0) && lane == 0) *odd = 1;
+            it += 2 * x.n;
+            nu++;
+            fine = __shfl_sync(0xffffffffu, (int)fine, 0);
+        }
+    } else if (warp == CHECKER) {
+        if (blockIdx.x == 0) {
+            int a, b, c, d;
+            for (int s = lane; s < p.nseq; s += 32)
+                if (!sequence(p, s, a, b, c, d)) *p.status = GALOIS_B200_E_BADARG;
+        }
+        int it = 0, nr = 0;
+        for (int r = 0; fine && x.find(p, f, unit_of_round(r), units, span, two_heads); r++) {
+            it += 2 * x.n;
+            if (!x.ragged()) continue;
+            fine = __all_sync(0xffffffffu, mbar_try_bounded(v_raw, nr & 1));
+            nr++;
+            if (!fine) break;
+            const int slot = (it - 1) % SLOTS, valid = x.nk - (x.n - 1) * PT;
+            uint4* v = reinterpret_cast<uint4*>(smem + L::KV + slot * L::TILE);  // [half][row][8 pieces]
+            for (int h = 0; h < HD / 64; h++)
+                for (int i = valid * 8 + lane; i < PT * 8; i += 32) v[h * PT * 8 + i] = make_uint4(0, 0, 0, 0);
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(full + slot);
         }
-    } else if (warp < 8) {
-        // ---- soft-max: thread = row
-        const int s = warp >> 2, row = threadIdx.x & 127;
-        const int first = tile * span + (two_heads ? 0 : s * PT), at = first + row, mine = n_tiles[s];
-        const int last = min(at + nk - nq, nk - 1);  // the last key that this row sees
-        const uint32_t s_at = tmem + s * PT + ((uint32_t)(warp & 3) << 21), o_at = tmem + 2 * PT + s * HD + ((uint32_t)(warp & 3) << 21);
+    } else {
+        // ---- soft-max: two threads per row, of 64 logits (and half of the result's columns) each
+        const int s = warp >> 3, half = (warp >> 2) & 1, row = (warp & 3) * 32 + lane;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+        const uint32_t s_at = tmem + s * PT + half * 64 + lanes, p_at = tmem + s * PT + half * 32 + lanes, o_at = tmem + 2 * PT + s * HD + half * (HD / 2) + lanes;
+        float* pair = reinterpret_cast<float*>(smem + L::PAIR) + s * 2 * PT;  // what the two threads of a row tell each other: maxima, sums
+        const int meet = 1 + s * 4 + (warp & 3);                               // their warps' barrier
         const float c = fmaxf(fabsf(p.scale) * 1.4426950408889634f, 1e-30f);  // not 0: a masked logit stays below all others
         const bool flip = p.scale < 0.0f;
-        float top = -INFINITY, l = 0.0f;  // what the probabilities refer to, their sum
-        for (int j = 0; j < mine; j++) {
-            fine = __all_sync(0xffffffffu, mbar_wait_bounded(s_full + s, j & 1));
-            if (!fine) break;
-            tc_after_sync();
-            // The logits are read twice, 32 at a time: 128 of them would not stay in registers.
-            const int see = j >= whole ? last - j * PT : PT;
-            float m0 = top, m1 = -INFINITY;
-            float x[2][32];
-            tc_ld32(s_at, reinterpret_cast<uint32_t*>(x[0]));
-#pragma unroll
-            for (int i = 0; i < PT / 32; i++) {
-                float* y = x[i & 1];
+        int nt = 0, nu = 0;
+        for (int r = 0;; r++) {
+            const int64_t u = unit_of_round(r);
+            // The unit is looked up here and again for the results: what describes it does not stay in registers.
+            f.start(p, span);
+            if (!x.find(p, f, u, units, span, two_heads)) break;
+            const int mine = s ? x.tiles1 : x.tiles0;
+            const int last = min(x.first + (two_heads ? 0 : s * PT) + row + x.nk - x.nq, x.nk - 1);  // the last key that this row sees
+            const int whole = max(0, x.first + x.nk - x.nq + 1) / PT;  // key tiles that every query sees whole
+            float top = -INFINITY, l = 0.0f;  // what the probabilities refer to; the sum of this thread's
+            for (int j = 0; j < mine; j++, nt++) {
+                fine = fine && __all_sync(0xffffffffu, mbar_try_bounded(s_full + s, nt & 1));  // both warps of a row go through all tiles
+                tc_after_sync();
+                float y[64];
+                tc_ld32(s_at, reinterpret_cast<uint32_t*>(y));
+                tc_ld32(s_at + 32, reinterpret_cast<uint32_t*>(y) + 32);
                 tc_wait_ld(reinterpret_cast<uint32_t*>(y));
-                tc_ld32(s_at + (i + 1) % (PT / 32) * 32, reinterpret_cast<uint32_t*>(x[(i + 1) & 1]));
-                if (flip || see < PT) {
+                tc_wait_ld(reinterpret_cast<uint32_t*>(y) + 32);
+                if (flip) {
 #pragma unroll
-                    for (int e = 0; e < 32; e++) y[e] = 32 * i + e <= see ? (flip ? -y[e] : y[e]) : -INFINITY;
+                    for (int e = 0; e < 64; e++) y[e] = -y[e];
                 }
+                if (j >= whole) {
+                    const int see = last - j * PT - half * 64;
 #pragma unroll
-                for (int e = 0; e < 32; e += 4) m0 = max3(m0, y[e], y[e + 1]), m1 = max3(m1, y[e + 2], y[e + 3]);
-            }
-            m0 = fmaxf(m0, m1);
-            const bool raise = (m0 - top) * c > 8.0f;  // also the first maximum of a row
-            if (__any_sync(0xffffffffu, raise)) {
-                const float to = raise ? m0 : top, keep = raise ? ex2((top - to) * c) : 1.0f;
-                top = to;
-                l *= keep;
-                if (j > 0) {
+                    for (int e = 0; e < 64; e++) y[e] = e <= see ? y[e] : -INFINITY;
+                }
+                float m0 = top, m1 = -INFINITY;
 #pragma unroll
-                    for (int i = 0; i < HD / 32; i++) {
-                        uint32_t o[32];
-                        tc_ld32(o_at + i * 32, o);
-                        tc_wait_ld(o);
+                for (int e = 0; e < 64; e += 4) m0 = max3(m0, y[e], y[e + 1]), m1 = max3(m1, y[e + 2], y[e + 3]);
+                m0 = max3(m0, m1, m1);
+                pair[half * PT + row] = m0;
+                // both halves' logits have been read when this is passed, so that the probabilities may be written over them
+                asm volatile("bar.sync %0, 64;" ::"r"(meet) : "memory");
+                const float m2 = pair[(half ^ 1) * PT + row];
+                m0 = max3(m0, m2, m2);
+                const bool raise = (m0 - top) * c > 8.0f || m0 != m0;  // also the first maximum of a row
+                if (__any_sync(0xffffffffu, raise)) {
+                    const float to = raise ? m0 : top, keep = raise ? ex2((top - to) * c) : 1.0f;
+                    top = to;
+                    l *= keep;
+                    if (j > 0) {
 #pragma unroll
-                        for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-                        tc_st32(o_at + i * 32, o);
+                        for (int i = 0; i < HD / 32; i++) {
+                            uint32_t o[16];
+                            tc_ld16(o_at + i * 16, o);
+                            tc_wait_ld16(o);
+#pragma unroll
+                            for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                            tc_st16(o_at + i * 16, o);
+                        }
                     }
                 }
-            }
-            const float shift = top == -INFINITY ? 0.0f : -top * c;
-            const uint64_t cc = f2_pack(c, c), sh = f2_pack(shift, shift);
-            uint64_t sum[2] = {0, 0};
+                const float shift = top == -INFINITY ? 0.0f : -top * c;
+                const uint64_t cc = f2_pack(c, c), sh = f2_pack(shift, shift);
+                uint64_t sum = 0;
 #pragma unroll
-            for (int i = 0; i < PT / 32; i++) {
-                float* y = x[i & 1];  // the first 32 were asked for above
-                tc_wait_ld(reinterpret_cast<uint32_t*>(y));
-                if (i + 1 < PT / 32) tc_ld32(s_at + (i + 1) * 32, reinterpret_cast<uint32_t*>(x[(i + 1) & 1]));
-                if (flip || see < PT) {
+                for (int i = 0; i < 2; i++) {
+                    uint32_t pk[16];
 #pragma unroll
-                    for (int e = 0; e < 32; e++) y[e] = 32 * i + e <= see ? (flip ? -y[e] : y[e]) : -INFINITY;
+                    for (int e = 0; e < 16; e++) {
+                        const uint64_t z = f2_fma(f2_pack(y[32 * i + 2 * e], y[32 * i + 2 * e + 1]), cc, sh);
+                        const float p0 = ex2(f2_low(z)), p1 = ex2(f2_high(z));
+                        sum = f2_add(sum, f2_pack(p0, p1));
+                        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(pk[e]) : "f"(p1), "f"(p0));
+                    }
+                    tc_st16(p_at + i * 16, pk);
                 }
-                uint32_t pk[16];
-#pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const uint64_t z = f2_fma(f2_pack(y[2 * e], y[2 * e + 1]), cc, sh);
-                    const float p0 = ex2(f2_low(z)), p1 = ex2(f2_high(z));
-                    sum[e & 1] = f2_add(sum[e & 1], f2_pack(p0, p1));
-                    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(pk[e]) : "f"(p1), "f"(p0));
-                }
-                tc_st16(s_at + i * 16, pk);
+                l += f2_low(sum) + f2_high(sum);
+                tc_wait_st();
+                tc_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_ready + s);
             }
-            sum[0] = f2_add(sum[0], sum[1]);
-            l += f2_low(sum[0]) + f2_high(sum[0]);
-            tc_wait_st();
-            tc_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(p_ready + s);
-        }
-        // ---- results
-        if (fine && mine > 0) {
-            fine = __all_sync(0xffffffffu, mbar_wait_bounded(o_done + s, 0));
+            // ---- results
+            f.start(p, span);
+            x.find(p, f, u, units, span, two_heads);
+            const int at = x.first + (two_heads ? 0 : s * PT) + row;
+            asm volatile("bar.sync %0, 64;" ::"r"(meet) : "memory");  // the other has read the last maximum
+            pair[half * PT + row] = l;
+            asm volatile("bar.sync %0, 64;" ::"r"(meet) : "memory");
+            l += pair[(half ^ 1) * PT + row];
+            asm volatile("bar.sync %0, 64;" ::"r"(meet) : "memory");  // and now the sum
+            if (mine > 0) {
+                fine = fine && __all_sync(0xffffffffu, mbar_try_bounded(o_done + s, nu & 1));
+                nu++;
+            }
             tc_after_sync();
-        }
-        if (fine) {
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            T* to = reinterpret_cast<T*>(p.out) + (int64_t)(two_heads ? head0 + s : head0) * p.o_head + (int64_t)(q0 + at) * p.o_tok;
+            const bool none = top == -INFINITY, live = fine && at < x.nq;  // no key, or none that counts
+            const float inv = none ? 0.0f : 1.0f / l;
+            const int head = two_heads ? x.head0 + s : x.head0;
+            T* out = reinterpret_cast<T*>(p.out) + (int64_t)head * p.o_head + (int64_t)(x.q0 + at - row) * p.o_tok;  // row 0's
+            T* to = out + (int64_t)row * p.o_tok + half * (HD / 2);
+            uint32_t odd = 0;  // sign bit: a result's exponent is all ones
 #pragma unroll
             for (int i = 0; i < HD / 32; i++) {
-                uint32_t o[32];
+                uint32_t o[16];
+                tc_ld16(o_at + i * 16, o);
+                tc_wait_ld16(o);
 #pragma unroll
-                for (int e = 0; e < 32; e++) o[e] = 0;
-                if (mine > 0) {
-                    tc_ld32(o_at + i * 32, o);
-                    tc_wait_ld(o);
+                for (int e = 0; e < 16; e++) {
+                    o[e] = none ? 0u : __float_as_uint(__uint_as_float(o[e]) * inv);
+                    odd |= (o[e] & 0x7f800000u) + 0x00800000u;
                 }
-                if (seq >= 0 && at < nq) {
-                    if constexpr (sizeof(T) == 4) {
+                if (!live) continue;
+                if constexpr (sizeof(T) == 4) {
 #pragma unroll
-                        for (int e = 0; e < 8; e++)
-                            reinterpret_cast<float4*>(to)[i * 8 + e] = l == 0.0f ? make_float4(0.f, 0.f, 0.f, 0.f)
-                                                                                 : make_float4(__uint_as_float(o[4 * e]) * inv, __uint_as_float(o[4 * e + 1]) * inv,
-                                                                                               __uint_as_float(o[4 * e + 2]) * inv, __uint_as_float(o[4 * e + 3]) * inv);
-                    } else {
-                        uint32_t h[16];
+                    for (int e = 0; e < 4; e++) reinterpret_cast<uint4*>(to)[i * 4 + e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                } else {
+                    uint32_t h[8];
 #pragma unroll
-                        for (int e = 0; e < 16; e++) {
-                            const float a = l == 0.0f ? 0.0f : __uint_as_float(o[2 * e]) * inv, b = l == 0.0f ? 0.0f : __uint_as_float(o[2 * e + 1]) * inv;
-                            asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h[e]) : "f"(b), "f"(a));
-                        }
+                    for (int e = 0; e < 8; e++) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h[e]) : "f"(__uint_as_float(o[2 * e + 1])), "f"(__uint_as_float(o[2 * e])));
 #pragma unroll
-                        for (int e = 0; e < 4; e++) reinterpret_cast<uint4*>(to)[i * 4 + e] = make_uint4(h[4 * e], h[4 * e + 1], h[4 * e + 2], h[4 * e + 3]);
-                    }
+                    for (int e = 0; e < 2; e++) reinterpret_cast<uint4*>(to)[i * 2 + e] = make_uint4(h[4 * e], h[4 * e + 1], h[4 * e + 2], h[4 * e + 3]);
+                }
+            }
+            tc_before_sync();
+            // this warp's half rows by the plain loop, where one of them is not finite
+            if (__any_sync(0xffffffffu, live && (odd >> 31))) {
+                for (int w = 0; w < 32; w++) {
+                    const int i = at - lane + w, key = i + x.nk - x.nq + 1;
+                    if (i < x.nq) prompt_row<HD, T>(p.q, p.k, p.v, x.q0 + i, x.k0, key, head, x.kh, p.scale, half, out + (int64_t)(row - lane + w) * p.o_tok);
                 }
             }
         }
@@ -386,14 +460,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (!fine && lane == 0) *p.status = GALOIS_B200_E_TIMEOUT;
     tc_before_sync();
     __syncthreads();
-    if (warp == 9) tc_dealloc(tmem, 512);
-    if (*odd) {
-        for (int r = warp; r < 2 * PT; r += THREADS / 32) {
-            const int s = r / PT, at = tile * span + (two_heads ? 0 : s * PT) + r % PT, h = two_heads ? head0 + s : head0;
-            if (at >= nq) continue;
-            prompt_row<HD, T>(p.q, p.k, p.v, q0 + at, k0, at + nk - nq + 1, h, kh, p.scale, reinterpret_cast<T*>(p.out) + h * p.o_head + (int64_t)(q0 + at) * p.o_tok);
-        }
-    }
+    if (warp == ISSUER) tc_dealloc(tmem, 512);
 }
 
 int check_rows16(galois_b200_ctx* ctx, const char* name, const void* p, const galois_dim* d, size_t elem) {
@@ -433,7 +500,7 @@ int prompt_attention(galois_b200_ctx* ctx, const void* q, const galois_dim* qd, 
     gb_on_device on(ctx);
     const rows16 qr{(const __half*)q, qd->nb[1], qd->nb[2]}, kr{(const __half*)k, kd->nb[1], kd->nb[2]}, vr{(const __half*)v, vd->nb[1], vd->nb[2]};
     const int group = heads / kv_heads, units = group % 2 == 0 ? heads / 2 : heads, span = group % 2 == 0 ? PT : 2 * PT;
-    // as many tiles as any lengths need: each sequence has at most one that is not full
+    // units as any lengths need, at most: each sequence has one tile at most that is not full
     const int64_t ctas = ((int64_t)tq / span + std::min(nseq, tq)) * units;
     if (ctas > 0x7fffffff) return gb_fail(ctx, GALOIS_B200_E_SHAPE, "prompt_attention: too many tokens");
     const prompt_args a{qr, kr, vr, q_starts, k_starts, nseq, tq, tk, heads, group, scale, dst, dd->nb[1], dd->nb[2], ctx->dev_status};
@@ -450,7 +517,7 @@ int prompt_attention(galois_b200_ctx* ctx, const void* q, const galois_dim* qd, 
         if (rc) return rc;
     }
     auto kern = qd->ne[0] == 64 ? prompt_attention_kernel<64, T> : prompt_attention_kernel<128, T>;
-    GB_CUDA(ctx, gb_launch(ctx, kern, dim3((unsigned)ctas), dim3(THREADS), qd->ne[0] == 64 ? plan<64>::TOTAL : plan<128>::TOTAL, a, maps[0], maps[1], maps[2]));
+    GB_CUDA(ctx, gb_launch(ctx, kern, dim3((unsigned)std::min<int64_t>(ctas, ctx->sm_count)), dim3(THREADS), qd->ne[0] == 64 ? plan<64>::TOTAL : plan<128>::TOTAL, a, maps[0], maps[1], maps[2]));
     GB_LAUNCHED(ctx, "prompt_attention");
     return 0;
 }

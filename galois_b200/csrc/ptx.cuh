@@ -59,6 +59,27 @@ __device__ __forceinline__ bool mbar_spin_bounded(uint64_t* bar, uint32_t parity
     }
     return true;
 }
+// One try_wait without a time hint: the hardware's own short suspension, from which a thread wakes sooner.
+__device__ __forceinline__ bool mbar_try(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// The bounded wait made of those.
+__device__ __forceinline__ bool mbar_try_bounded(uint64_t* bar, uint32_t parity) {
+    if (mbar_try(bar, parity)) return true;
+    const long long t0 = clock64();
+    while (!mbar_try(bar, parity)) {
+        if (clock64() - t0 > (1ll << 32)) return false;
+    }
+    return true;
+}
 // 1-D bulk copy global -> this CTA's shared memory, completing on an mbarrier.  Both addresses
 // 16-byte aligned, size a multiple of 16 bytes.  No multicast.
 __device__ __forceinline__ void bulk_g2s(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {

@@ -45,6 +45,12 @@ __device__ __forceinline__ void tc_wait_ld(uint32_t* r) {
                  :
                  : "memory");
 }
+__device__ __forceinline__ void tc_wait_ld16(uint32_t* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // 32 lanes x 32 (16) consecutive 32-bit columns: thread i of the warp gets lane (base + i)
 __device__ __forceinline__ void tc_ld32(uint32_t taddr, uint32_t* r) {

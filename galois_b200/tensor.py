@@ -256,8 +256,8 @@ class Tensor:
     def c_dim(self):
         """The C form of ``dim()`` by reference, built once: a tensor's shape and strides do not change."""
         if self._c_dim is None:
-            self._c_dim = self._dim.c_struct()
-        return C.byref(self._c_dim)
+            self._c_dim = C.byref(self._dim.c_struct())
+        return self._c_dim
 
     def shape(self):
         return self._dim.shape[: self._dim.n_dims]
