@@ -15,33 +15,49 @@ constexpr float Q8_MAX = 3.402823466e38f;
 
 __device__ __forceinline__ float tame(float x) { return x != x ? 0.0f : fminf(fmaxf(x, -Q8_MAX), Q8_MAX); }
 
+// 16 bytes of a row of new numbers: 4 f32 or 8 F16.
 template <typename T>
-__device__ __forceinline__ float4 load4(const T* p);
+struct piece;
 template <>
-__device__ __forceinline__ float4 load4<float>(const float* p) {
-    return *reinterpret_cast<const float4*>(p);
-}
+struct piece<float> {
+    static constexpr int N = 4;
+    uint4 w;
+    // the largest magnitude's bits; 0x7f800000 and above: not finite
+    __device__ __forceinline__ uint32_t top() const { return max(max(w.x & 0x7fffffffu, w.y & 0x7fffffffu), max(w.z & 0x7fffffffu, w.w & 0x7fffffffu)); }
+    __device__ __forceinline__ float4 get(int) const { return make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w)); }
+    static __device__ __forceinline__ float magnitude(uint32_t t) { return __uint_as_float(t); }
+};
 template <>
-__device__ __forceinline__ float4 load4<__half>(const __half* p) {
-    const uint2 w = *reinterpret_cast<const uint2*>(p);
-    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
-    return make_float4(a.x, a.y, b.x, b.y);
-}
+struct piece<__half> {
+    static constexpr int N = 8;
+    uint4 w;
+    __device__ __forceinline__ uint32_t top() const {
+        const uint32_t m = __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
+        return max(m & 0xffffu, m >> 16);
+    }
+    __device__ __forceinline__ float4 get(int i) const {
+        const uint32_t u = i ? w.z : w.x, v = i ? w.w : w.y;
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u)), b = __half22float2(*reinterpret_cast<const __half2*>(&v));
+        return make_float4(a.x, a.y, b.x, b.y);
+    }
+    static __device__ __forceinline__ float magnitude(uint32_t t) { return __half2float(__ushort_as_half((unsigned short)t)); }
+};
+
 // ---------------------------------------------------------------- append
 // A CTA of 128 threads looks at `tile` packed tokens of one head, of the keys (z = 0) or the values (z = 1).  Each
 // token there that is the first new one of its block leads the block: the CTA takes all new rows of that block into
-// registers (a lane holds 4 numbers of a row), finds the largest magnitude, settles the scale and writes.  A block has
-// one leader, so no two CTAs write the same rows or scale.
+// registers (16 bytes of a row a lane), finds the largest magnitude, settles the scale and writes.  A block has one
+// leader, so no two CTAs write the same rows or scale.
 template <typename T, int HD>
 __global__ void __launch_bounds__(128) cache_append_kernel(const T* __restrict__ k, int64_t k_head, int64_t k_tok, const T* __restrict__ v,
                                                            int64_t v_head, int64_t v_tok, const int32_t* __restrict__ starts,
                                                            const int32_t* __restrict__ pos, int nseq, int tokens, int tile, gb_cache_view c,
                                                            int* __restrict__ status) {
     gb_pdl_entry();
-    constexpr int LPR = HD / 4, RPP = 128 / LPR, N = GB_CACHE_BLOCK / RPP;  // lanes per row, rows per pass, passes
-    __shared__ float red[4];
+    constexpr int V = piece<T>::N, W = V / 4, LPR = HD / V, RPP = 128 / LPR, N = GB_CACHE_BLOCK / RPP;  // numbers and words a lane, lanes a row, rows a pass, passes
+    __shared__ uint32_t red[4];
     const int head = blockIdx.y, warp = threadIdx.x >> 5;
-    const int row0 = threadIdx.x / LPR, col = (threadIdx.x % LPR) * 4;
+    const int row0 = threadIdx.x / LPR, col = (threadIdx.x % LPR) * V;
     const T* x = (blockIdx.z ? v + head * v_head : k + head * k_head) + col;
     const int64_t x_tok = blockIdx.z ? v_tok : k_tok;
     int8_t* q = (blockIdx.z ? c.v : c.k) + head * c.head + col;
@@ -62,39 +78,64 @@ __global__ void __launch_bounds__(128) cache_append_kernel(const T* __restrict__
             continue;
         }
         const int lo = p % GB_CACHE_BLOCK, hi = min(GB_CACHE_BLOCK, lo + end - t);
-        float4 r[N];
-        float top = 0.0f;
+        piece<T> r[N];
+        const T* from = x + (int64_t)(t + row0 - lo) * x_tok;
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            const int row = row0 + i * RPP;
-            r[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (row >= lo && row < hi) r[i] = load4(x + (int64_t)(t + row - lo) * x_tok);
-        }
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            r[i] = make_float4(tame(r[i].x), tame(r[i].y), tame(r[i].z), tame(r[i].w));
-            top = fmaxf(top, fmaxf(fmaxf(fabsf(r[i].x), fabsf(r[i].y)), fmaxf(fabsf(r[i].z), fabsf(r[i].w))));
+        for (int i = 0; i < N; i++, from += RPP * x_tok) {
+            r[i].w = make_uint4(0, 0, 0, 0);
+            if (row0 + i * RPP >= lo && row0 + i * RPP < hi) r[i].w = *reinterpret_cast<const uint4*>(from);
         }
         float* scale = scales + s * c.s_seq + block;
         const float held = lo > 0 ? *scale : 0.0f;
-        top = gb_warp_max(top);
+        uint32_t bits = 0;
+#pragma unroll
+        for (int i = 0; i < N; i++) bits = max(bits, r[i].top());
+        bits = __reduce_max_sync(0xffffffffu, bits);
         __syncthreads();  // the last block's maxima have been read
-        if ((threadIdx.x & 31) == 0) red[warp] = top;
+        if ((threadIdx.x & 31) == 0) red[warp] = bits;
         __syncthreads();  // also: every thread has read the held scale
-        float d = fmaxf(__fdiv_rn(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), 127.0f), held);
+        float top = piece<T>::magnitude(max(max(red[0], red[1]), max(red[2], red[3])));
+        const bool odd = !(top <= Q8_MAX);  // something is not finite: infinities count as the largest number, NaN as 0
+        if (odd) {
+            float m = 0.0f;
+#pragma unroll
+            for (int i = 0; i < N; i++)
+#pragma unroll
+                for (int j = 0; j < W; j++) {
+                    const float4 f = r[i].get(j);
+                    m = fmaxf(m, fmaxf(fmaxf(fabsf(tame(f.x)), fabsf(tame(f.y))), fmaxf(fabsf(tame(f.z)), fabsf(tame(f.w)))));
+                }
+            const uint32_t u = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
+            __syncthreads();
+            if ((threadIdx.x & 31) == 0) red[warp] = u;
+            __syncthreads();
+            top = __uint_as_float(max(max(red[0], red[1]), max(red[2], red[3])));
+        }
+        float d = fmaxf(__fdiv_rn(top, 127.0f), held);
         if (!(d >= Q8_TINY)) d = 0.0f;
         if (threadIdx.x == 0) *scale = d;
-        int8_t* out = q + s * c.seq + (int64_t)block * GB_CACHE_BLOCK * c.tok;
-        const float rd = d > 0.0f ? __fdiv_rn(1.0f, d) : 0.0f, ratio = d > 0.0f ? __fdiv_rn(held, d) : 0.0f;
+        int8_t* to = q + s * c.seq + (int64_t)(block * GB_CACHE_BLOCK + row0) * c.tok;
+        const gb_around by = gb_make_around(d > 0.0f ? __fdiv_rn(1.0f, d) : 0.0f);
 #pragma unroll
-        for (int i = 0; i < N; i++) {
+        for (int i = 0; i < N; i++, to += RPP * c.tok) {
             const int row = row0 + i * RPP;
-            uint32_t* to = reinterpret_cast<uint32_t*>(out + row * c.tok);
+            uint32_t w[W];
             if (row >= lo && row < hi) {
-                *to = d > 0.0f ? gb_q8_round4(r[i], d, rd) : 0u;
+#pragma unroll
+                for (int j = 0; j < W; j++) {
+                    float4 f = r[i].get(j);
+                    if (odd) f = make_float4(tame(f.x), tame(f.y), tame(f.z), tame(f.w));
+                    w[j] = d > 0.0f ? gb_q8_round4(f, d, by) : 0u;
+                }
             } else if (row < lo && d != held) {
-                *to = gb_q8_rescale4(*to, held, d, ratio);
+                const gb_around ratio = gb_make_around(d > 0.0f ? __fdiv_rn(held, d) : 0.0f);
+#pragma unroll
+                for (int j = 0; j < W; j++) w[j] = gb_q8_rescale4(reinterpret_cast<const uint32_t*>(to)[j], held, d, ratio);
+            } else {
+                continue;
             }
+            if constexpr (W == 1) *reinterpret_cast<uint32_t*>(to) = w[0];
+            else *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
         }
         t = min(next, end);
     }
@@ -115,41 +156,59 @@ __global__ void __launch_bounds__(128) cache_read_kernel(gb_cache_view c, const 
     const float* scales = (blockIdx.z ? c.vs : c.ks) + head * c.s_head;
     T* y = (blockIdx.z ? v + head * v_head : k + head * k_head) + col;
     const int64_t y_tok = blockIdx.z ? v_tok : k_tok;
-    const int t0 = (int)blockIdx.x * READ_ROWS + threadIdx.x / LPR;
-    int s = gb_find_seq(starts, nseq, (int)blockIdx.x * READ_ROWS);
+    const int tile = (int)blockIdx.x * READ_ROWS, t0 = tile + threadIdx.x / LPR;
+    int s = gb_find_seq(starts, nseq, tile);
     int begin = 0, end = 0, p0 = 0;
     if (s < nseq) begin = starts[s], end = starts[s + 1], p0 = pos[s];
     uint32_t w[N][W];
     float d[N];
     bool live[N];
+    if (s < nseq && begin >= 0 && begin <= tile && end >= tile + READ_ROWS && end <= tokens && p0 >= 0 && p0 <= c.ctx - READ_ROWS - (tile - begin)) {
+        // all rows of one sequence
+        const int p = p0 + (t0 - begin);
+        const int8_t* from = q + s * c.seq + p * c.tok;
+        const float* scale = scales + s * c.s_seq;
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-        const int t = t0 + i * RPP;
-        live[i] = false;
-        while (s < nseq && end <= t) {
-            if (++s < nseq) begin = end, end = starts[s + 1], p0 = pos[s];
-        }
-        if (t < tokens && s < nseq) {
-            if (begin < 0 || begin > t || end > tokens || p0 < 0 || p0 >= c.ctx - (t - begin)) {
-                *status = GALOIS_B200_E_BADARG;
+        for (int i = 0; i < N; i++, from += RPP * c.tok) {
+            live[i] = true;
+            if constexpr (W == 1) {
+                w[i][0] = *reinterpret_cast<const uint32_t*>(from);
             } else {
-                const int p = p0 + (t - begin);
-                live[i] = true;
-                const int8_t* from = q + s * c.seq + p * c.tok;
-                if constexpr (W == 1) {
-                    w[i][0] = *reinterpret_cast<const uint32_t*>(from);
+                const uint2 u = *reinterpret_cast<const uint2*>(from);
+                w[i][0] = u.x, w[i][1] = u.y;
+            }
+            d[i] = scale[(p + i * RPP) / GB_CACHE_BLOCK];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int t = t0 + i * RPP;
+            live[i] = false;
+            while (s < nseq && end <= t) {
+                if (++s < nseq) begin = end, end = starts[s + 1], p0 = pos[s];
+            }
+            if (t < tokens && s < nseq) {
+                if (begin < 0 || begin > t || end > tokens || p0 < 0 || p0 >= c.ctx - (t - begin)) {
+                    *status = GALOIS_B200_E_BADARG;
                 } else {
-                    const uint2 u = *reinterpret_cast<const uint2*>(from);
-                    w[i][0] = u.x, w[i][1] = u.y;
+                    const int p = p0 + (t - begin);
+                    live[i] = true;
+                    const int8_t* from = q + s * c.seq + p * c.tok;
+                    if constexpr (W == 1) {
+                        w[i][0] = *reinterpret_cast<const uint32_t*>(from);
+                    } else {
+                        const uint2 u = *reinterpret_cast<const uint2*>(from);
+                        w[i][0] = u.x, w[i][1] = u.y;
+                    }
+                    d[i] = scales[s * c.s_seq + p / GB_CACHE_BLOCK];
                 }
-                d[i] = scales[s * c.s_seq + p / GB_CACHE_BLOCK];
             }
         }
     }
+    T* to = y + (int64_t)t0 * y_tok;
 #pragma unroll
-    for (int i = 0; i < N; i++) {
+    for (int i = 0; i < N; i++, to += RPP * y_tok) {
         if (!live[i]) continue;
-        T* to = y + (int64_t)(t0 + i * RPP) * y_tok;
         float4 f[W];
 #pragma unroll
         for (int j = 0; j < W; j++) {
@@ -316,25 +375,31 @@ __global__ void __launch_bounds__(128) cache_gather_kernel(gb_cache_view c, gb_c
     const int8_t* q = (values ? c.v : c.k) + head * c.head + s * c.seq;
     int8_t* out = (values ? o.v : o.k) + head * o.head + s * o.seq + (int64_t)block * GB_CACHE_BLOCK * o.tok;
     const int src = lane < m ? idx[lane] : 0;  // every warp holds all 32
+    const int col = (threadIdx.x % LPR) * 16;
+    uint4 w[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const int row = threadIdx.x / LPR + i * RPP;
+        const int from = __shfl_sync(0xffffffffu, src, row & 31);
+        w[i] = make_uint4(0, 0, 0, 0);
+        if (row < m) w[i] = *reinterpret_cast<const uint4*>(q + from * c.tok + col);
+    }
     const float ds = lane < m ? scales[src / GB_CACHE_BLOCK] : 0.0f;
     float d = gb_warp_max(ds);
     if (!(d >= Q8_TINY)) d = 0.0f;
     if (threadIdx.x == 0) ((values ? o.vs : o.ks) + head * o.s_head + s * o.s_seq)[block] = d;
     const float ratio = d > 0.0f ? __fdiv_rn(ds, d) : 0.0f;
-    const int col = (threadIdx.x % LPR) * 16;
 #pragma unroll
     for (int i = 0; i < N; i++) {
         const int row = threadIdx.x / LPR + i * RPP;
-        const int from = __shfl_sync(0xffffffffu, src, row & 31);
-        const float d0 = __shfl_sync(0xffffffffu, ds, row & 31), r = __shfl_sync(0xffffffffu, ratio, row & 31);
+        const float d0 = __shfl_sync(0xffffffffu, ds, row & 31);
+        const gb_around r = gb_make_around(__shfl_sync(0xffffffffu, ratio, row & 31));
         if (row >= m) continue;
-        uint4 w = *reinterpret_cast<const uint4*>(q + from * c.tok + col);
         if (d0 != d) {
-            uint32_t* p = reinterpret_cast<uint32_t*>(&w);
-#pragma unroll
-            for (int j = 0; j < 4; j++) p[j] = d > 0.0f ? gb_q8_rescale4(p[j], d0, d, r) : 0u;
+            if (d > 0.0f) w[i] = make_uint4(gb_q8_rescale4(w[i].x, d0, d, r), gb_q8_rescale4(w[i].y, d0, d, r), gb_q8_rescale4(w[i].z, d0, d, r), gb_q8_rescale4(w[i].w, d0, d, r));
+            else w[i] = make_uint4(0, 0, 0, 0);
         }
-        *reinterpret_cast<uint4*>(out + row * o.tok + col) = w;
+        *reinterpret_cast<uint4*>(out + row * o.tok + col) = w[i];
     }
 }
 

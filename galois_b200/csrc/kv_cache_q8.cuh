@@ -71,28 +71,35 @@ __device__ __forceinline__ int gb_find_seq(const int32_t* __restrict__ starts, i
     return __reduce_add_sync(0xffffffffu, c);
 }
 
-// Four whole numbers, each round-half-even of the exact quotient x / d, as bytes; rd = 1 / d rounded, |x| at most 127.5 d.
-// x * rd is off by less than 2^-16, so its rounding (by adding 1.5 * 2^23, whose last bits are then the whole number) is
-// wrong only next to a border k + 1/2.  There the sign of x - (k + 1/2) d decides, which one fused multiply-add gives
-// exactly (d is not below 2^-100).
+// A quotient x / d is rounded to a whole number (half to even) by adding 1.5 * 2^23 to x * (1 / d): the sum's last bits are
+// the number.  1 / d is not exact, so it is taken a little too small and a little too large: where both give the same
+// number it is the exact quotient's, else a border k + 1/2 lies next to it and is compared with in full.
 #define GB_ROUND 12582912.0f
-__device__ __forceinline__ float gb_q8_border(float y, float x, float d) {
-    float q = y - GB_ROUND;
+struct gb_around {
+    float lo, hi;
+};
+__device__ __forceinline__ gb_around gb_make_around(float r) { return gb_around{__fmul_rn(r, 1.0f - 0x1p-22f), __fmul_rn(r, 1.0f + 0x1p-22f)}; }
+__device__ __forceinline__ uint32_t gb_low_bytes(float a, float b, float c, float d) {
+    return __byte_perm(__byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040), __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040), 0x5410);
+}
+__device__ __forceinline__ uint32_t gb_bytes_of(float4 x, float r) {
+    return gb_low_bytes(fmaf(x.x, r, GB_ROUND), fmaf(x.y, r, GB_ROUND), fmaf(x.z, r, GB_ROUND), fmaf(x.w, r, GB_ROUND));
+}
+// The whole number next to q that is nearest to x / d, by the signs of x - (q -+ 1/2) d, which one fused multiply-add gives
+// exactly (d is not below 2^-100).
+__device__ __forceinline__ float gb_q8_border(float x, float d, float r) {
+    float q = rintf(__fmul_rn(x, r));
     const float lo = fmaf(-(q - 0.5f), d, x), hi = fmaf(-(q + 0.5f), d, x);
     const bool odd = ((int)q) & 1;
     if (lo < 0.0f || (lo == 0.0f && odd)) q -= 1.0f;
     else if (hi > 0.0f || (hi == 0.0f && odd)) q += 1.0f;
     return fminf(fmaxf(q, -127.0f), 127.0f) + GB_ROUND;
 }
-__device__ __forceinline__ uint32_t gb_low_bytes(float a, float b, float c, float d) {
-    return __byte_perm(__byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040), __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040), 0x5410);
-}
-__device__ __forceinline__ uint32_t gb_q8_round4(float4 x, float d, float rd) {
-    float y[4] = {fmaf(x.x, rd, GB_ROUND), fmaf(x.y, rd, GB_ROUND), fmaf(x.z, rd, GB_ROUND), fmaf(x.w, rd, GB_ROUND)};
-    const float far = fmaxf(fmaxf(fabsf(fmaf(x.x, rd, GB_ROUND - y[0])), fabsf(fmaf(x.y, rd, GB_ROUND - y[1]))),
-                            fmaxf(fabsf(fmaf(x.z, rd, GB_ROUND - y[2])), fabsf(fmaf(x.w, rd, GB_ROUND - y[3]))));
-    if (far > 0.5f - 0x1p-15f) y[0] = gb_q8_border(y[0], x.x, d), y[1] = gb_q8_border(y[1], x.y, d), y[2] = gb_q8_border(y[2], x.z, d), y[3] = gb_q8_border(y[3], x.w, d);
-    return gb_low_bytes(y[0], y[1], y[2], y[3]);
+// Four numbers as bytes; r: around 1 / d, |x| at most 127.5 d.
+__device__ __forceinline__ uint32_t gb_q8_round4(float4 x, float d, const gb_around& r) {
+    const uint32_t a = gb_bytes_of(x, r.lo);
+    if (a == gb_bytes_of(x, r.hi)) return a;
+    return gb_low_bytes(gb_q8_border(x.x, d, r.lo), gb_q8_border(x.y, d, r.lo), gb_q8_border(x.z, d, r.lo), gb_q8_border(x.w, d, r.lo));
 }
 // The bytes of w as f32.
 __device__ __forceinline__ float4 gb_q8_float4(uint32_t w) {
@@ -100,23 +107,20 @@ __device__ __forceinline__ float4 gb_q8_float4(uint32_t w) {
     return make_float4(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440)) - 8388736.0f, __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7441)) - 8388736.0f,
                        __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7442)) - 8388736.0f, __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7443)) - 8388736.0f);
 }
-// The same rounding of q0 * d0 / d for four whole numbers that move to a larger scale; r = d0 / d rounded.  The product has
-// 32 bits, so next to a border the two sides are compared in 64 bits, where both are exact.
-__device__ __forceinline__ float gb_q8_border64(float y, float q0, float d0, float d) {
-    float q = y - GB_ROUND;
+// The same of q0 * d0 / d for four whole numbers that move to a larger scale; r: around d0 / d.  The product has 32 bits, so
+// next to a border the two sides are compared in 64 bits, where both are exact.
+__device__ __forceinline__ float gb_q8_border64(float q0, float d0, float d, float r) {
+    float q = rintf(__fmul_rn(q0, r));
     const double x = (double)q0 * (double)d0, lo = x - ((double)q - 0.5) * (double)d, hi = x - ((double)q + 0.5) * (double)d;
     const bool odd = ((int)q) & 1;
     if (lo < 0.0 || (lo == 0.0 && odd)) q -= 1.0f;
     else if (hi > 0.0 || (hi == 0.0 && odd)) q += 1.0f;
     return fminf(fmaxf(q, -127.0f), 127.0f) + GB_ROUND;
 }
-__device__ __forceinline__ uint32_t gb_q8_rescale4(uint32_t w, float d0, float d, float r) {
+__device__ __forceinline__ uint32_t gb_q8_rescale4(uint32_t w, float d0, float d, const gb_around& r) {
     const float4 x = gb_q8_float4(w);
-    float y[4] = {fmaf(x.x, r, GB_ROUND), fmaf(x.y, r, GB_ROUND), fmaf(x.z, r, GB_ROUND), fmaf(x.w, r, GB_ROUND)};
-    const float far = fmaxf(fmaxf(fabsf(fmaf(x.x, r, GB_ROUND - y[0])), fabsf(fmaf(x.y, r, GB_ROUND - y[1]))),
-                            fmaxf(fabsf(fmaf(x.z, r, GB_ROUND - y[2])), fabsf(fmaf(x.w, r, GB_ROUND - y[3]))));
-    if (far > 0.5f - 0x1p-15f)
-        y[0] = gb_q8_border64(y[0], x.x, d0, d), y[1] = gb_q8_border64(y[1], x.y, d0, d), y[2] = gb_q8_border64(y[2], x.z, d0, d), y[3] = gb_q8_border64(y[3], x.w, d0, d);
-    return gb_low_bytes(y[0], y[1], y[2], y[3]);
+    const uint32_t a = gb_bytes_of(x, r.lo);
+    if (a == gb_bytes_of(x, r.hi)) return a;
+    return gb_low_bytes(gb_q8_border64(x.x, d0, d, r.lo), gb_q8_border64(x.y, d0, d, r.lo), gb_q8_border64(x.z, d0, d, r.lo), gb_q8_border64(x.w, d0, d, r.lo));
 }
 #endif
