@@ -38,19 +38,17 @@ struct rows16 {  // an F16 {head_dim, heads, tokens} operand
     int64_t head, tok;
 };
 
-// Half of one query row's result by one warp: a lane holds HD / 32 numbers of the query, HD / 64 of the result.
+// One query row by one warp: a lane holds HD / 32 numbers.
 template <int HD, typename T>
-__device__ __noinline__ void prompt_row(const rows16& q, const rows16& k, const rows16& v, int t, int k0, int n, int h, int kh, float scale, int half, T* out) {
-    constexpr int E = HD / 32, EO = HD / 64;
-    const int lane = threadIdx.x & 31, col = half * (HD / 2) + lane * EO;
-    float qr[E], o[EO], m = -INFINITY, l = 0.0f;
+__device__ __noinline__ void prompt_row(const rows16& q, const rows16& k, const rows16& v, int t, int k0, int n, int h, int kh, float scale, T* out) {
+    constexpr int E = HD / 32;
+    const int lane = threadIdx.x & 31;
+    float qr[E], o[E], m = -INFINITY, l = 0.0f;
 #pragma unroll
-    for (int e = 0; e < E; e++) qr[e] = __half2float(q.p[h * q.head + t * q.tok + lane * E + e]) * scale;
-#pragma unroll
-    for (int e = 0; e < EO; e++) o[e] = 0.0f;
+    for (int e = 0; e < E; e++) qr[e] = __half2float(q.p[h * q.head + t * q.tok + lane * E + e]) * scale, o[e] = 0.0f;
     for (int j = 0; j < n; j++) {
         const __half* kr = k.p + kh * k.head + (int64_t)(k0 + j) * k.tok + lane * E;
-        const __half* vr = v.p + kh * v.head + (int64_t)(k0 + j) * v.tok + col;
+        const __half* vr = v.p + kh * v.head + (int64_t)(k0 + j) * v.tok + lane * E;
         float x = 0.0f;
 #pragma unroll
         for (int e = 0; e < E; e++) x = fmaf(qr[e], __half2float(kr[e]), x);
@@ -59,24 +57,24 @@ __device__ __noinline__ void prompt_row(const rows16& q, const rows16& k, const 
         m = top;
         l = l * keep + p;
 #pragma unroll
-        for (int e = 0; e < EO; e++) o[e] = fmaf(p, __half2float(vr[e]), o[e] * keep);
+        for (int e = 0; e < E; e++) o[e] = fmaf(p, __half2float(vr[e]), o[e] * keep);
     }
 #pragma unroll
-    for (int e = 0; e < EO; e++) {
+    for (int e = 0; e < E; e++) {
         const float x = l == 0.0f ? 0.0f : o[e] / l;
-        if constexpr (sizeof(T) == 4) out[col + e] = x;
-        else out[col + e] = __float2half_rn(x);
+        if constexpr (sizeof(T) == 4) out[lane * E + e] = x;
+        else out[lane * E + e] = __float2half_rn(x);
     }
 }
 
 constexpr int PT = 128;      // rows of a tile of queries, of keys, of values
-constexpr int LOADER = 16, ISSUER = 17, CHECKER = 18;  // warps behind the soft-max's
-constexpr int THREADS = 19 * 32;
+constexpr int LOADER = 8, ISSUER = 9, CLEARER = 10;  // warps behind the soft-max's
+constexpr int THREADS = 11 * 32;
 template <int HD>
 struct plan {
     static constexpr uint32_t TILE = PT * HD * 2, HALF = PT * 128;  // bytes of a tile; of its first 64 columns
     static constexpr int SLOTS = HD == 128 ? 5 : 12;                // tiles of keys and values in shared memory
-    static constexpr uint32_t Q = 0, KV = 2 * TILE, BARS = KV + SLOTS * TILE, PAIR = BARS + 320, TOTAL = PAIR + 2 * 2 * PT * 4;
+    static constexpr uint32_t Q = 0, KV = 2 * TILE, BARS = KV + SLOTS * TILE, TOTAL = BARS + 320;
     static_assert(TOTAL <= 227 * 1024, "shared memory");
 };
 struct prompt_args {
@@ -188,7 +186,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         tma_prefetch_map(&q_map), tma_prefetch_map(&k_map), tma_prefetch_map(&v_map);
         mbar_init(q_full, 1), mbar_init(q_free, 1), mbar_init(v_raw, 1);
         for (int i = 0; i < SLOTS; i++) mbar_init(full + i, 1), mbar_init(empty + i, 1);
-        for (int i = 0; i < 2; i++) mbar_init(s_full + i, 1), mbar_init(p_ready + i, 8), mbar_init(o_done + i, 1);
+        for (int i = 0; i < 2; i++) mbar_init(s_full + i, 1), mbar_init(p_ready + i, 4), mbar_init(o_done + i, 1);
         fence_mbarrier_init_cluster();
     }
     if (warp == ISSUER) {
@@ -225,7 +223,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     const int slot = it % SLOTS;
                     if (it >= SLOTS) fine = mbar_try_bounded(empty + slot, (it / SLOTS - 1) & 1);
                     if (!fine) break;
-                    // a last tile of values that warp 18 has to clear arrives at a barrier of its own; it passes the tile on
+                    // a last tile of values that warp 10 has to clear arrives at a barrier of its own; it passes the tile on
                     uint64_t* bar = i == 2 * x.n - 1 && x.ragged() ? v_raw : full + slot;
                     mbar_expect_tx(bar, L::TILE);
                     for (int h = 0; h < HD / 64; h++)
@@ -247,61 +245,70 @@ __global__ void __launch_bounds__(THREADS, 1)
         // f32 sums, F16 operands; logits: keys as they are; results: values with the contraction along their rows
         const uint32_t idesc_s = (1u << 4) | ((uint32_t)(PT >> 3) << 17) | ((uint32_t)(PT >> 4) << 24);
         const uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(PT >> 4) << 24);
-        const uint32_t q_at = smem_u32(smem + L::Q), kv_at = smem_u32(smem + L::KV);
-        int it = 0, nu = 0;
-        int ready[2] = {0, 0};  // tiles of each query tile whose probabilities have been waited for
-        auto logits = [&](int s, int slot) {
-            const uint32_t k_at = kv_at + (uint32_t)slot * L::TILE;
+        // The whole warp goes through this, and one thread of it issues (see tc_elect).
+        const uint32_t lead = tc_elect();
+        const uint64_t q_desc = tc_desc(smem_u32(smem + L::Q), 16, 1024, 128), k_desc = tc_desc(smem_u32(smem + L::KV), 16, 1024, 128),
+                       v_desc = tc_desc(smem_u32(smem + L::KV), L::HALF, 1024, 128);
+        int slot = 0;
+        uint32_t parity = 0, q_parity = 0;   // of the ring's round, of the next queries
+        uint32_t ready[2] = {0, 0};          // of the next probabilities of each query tile
+        auto next = [&]() {
+            if (++slot == SLOTS) slot = 0, parity ^= 1;
+        };
+        auto wait = [&](uint64_t* bar, uint32_t phase) { return __all_sync(0xffffffffu, mbar_try_bounded(bar, phase)) != 0; };
+        auto logits = [&](int s) {  // of the keys in `slot`
+            const uint64_t a = q_desc + (uint32_t)(s * (L::TILE >> 4)), b = k_desc + (uint32_t)(slot * (L::TILE >> 4));
 #pragma unroll
             for (int kk = 0; kk < HD / 16; kk++) {
-                const uint32_t off = (kk / 4) * L::HALF + (kk % 4) * 32;
-                tc_mma_f16_ss(tmem + s * PT, tc_desc(q_at + s * L::TILE + off, 16, 1024, 128), tc_desc(k_at + off, 16, 1024, 128), idesc_s, kk > 0);
+                constexpr uint32_t H = L::HALF >> 4;
+                tc_mma_f16_ss(tmem + s * PT, a + (kk / 4 * H + kk % 4 * 2), b + (kk / 4 * H + kk % 4 * 2), idesc_s, kk > 0, lead);
             }
-            tc_commit(s_full + s);
+            tc_commit(s_full + s, lead);
         };
         for (int r = 0; fine && x.find(p, f, unit_of_round(r), units, span, two_heads); r++) {
             if (x.n == 0) continue;
-            if (lane == 0) {
-                const int tiles[2] = {x.tiles0, x.tiles1};
-                fine = mbar_try_bounded(q_full, nu & 1) && mbar_try_bounded(full + it % SLOTS, (it / SLOTS) & 1);
-                if (fine) {
-                    for (int s = 0; s < 2; s++)
-                        if (tiles[s] > 0) logits(s, it % SLOTS);
-                    tc_commit(empty + it % SLOTS);
-                    if (x.n == 1) tc_commit(q_free);
-                }
-                for (int j = 0; j < x.n && fine; j++) {
-                    const int vi = it + 2 * j + 1, vs = vi % SLOTS, ki = vi + 1, ks = ki % SLOTS;
-                    fine = mbar_try_bounded(full + vs, (vi / SLOTS) & 1);
-                    bool keys = false;  // the next keys have arrived
-                    for (int s = 0; s < 2 && fine; s++) {
-                        if (j >= tiles[s]) continue;
-                        fine = mbar_try_bounded(p_ready + s, ready[s] & 1);
-                        ready[s]++;
-                        if (!fine) break;
-                        tc_after_sync();
+            fine = wait(q_full, q_parity) && wait(full + slot, parity);
+            q_parity ^= 1;
+            if (!fine) break;
+            if (x.tiles0 > 0) logits(0);
+            if (x.tiles1 > 0) logits(1);
+            tc_commit(empty + slot, lead);
+            if (x.n == 1) tc_commit(q_free, lead);
+            for (int j = 0; j < x.n && fine; j++) {
+                next();
+                const int vs = slot;
+                fine = wait(full + vs, parity);
+                const bool more = j + 1 < x.n;
+                if (more) next();
+                bool keys = false;  // the next keys have arrived
 #pragma unroll
-                        for (int kk = 0; kk < PT / 16; kk++)
-                            tc_mma_f16_ts(tmem + 2 * PT + s * HD, tmem + s * PT + kk * 8, tc_desc(kv_at + vs * L::TILE + kk * 2048, L::HALF, 1024, 128), idesc_o, j > 0 || kk > 0);
-                        if (s == 1 || j >= tiles[1]) tc_commit(empty + vs);
-                        if (j + 1 < tiles[s]) {
-                            if (!keys) fine = mbar_try_bounded(full + ks, (ki / SLOTS) & 1);
-                            if (!fine) break;
-                            keys = true;
-                            logits(s, ks);
-                        } else {
-                            tc_commit(o_done + s);
-                        }
+                for (int s = 0; s < 2; s++) {
+                    const int tiles = s ? x.tiles1 : x.tiles0;
+                    if (j >= tiles || !fine) continue;
+                    fine = wait(p_ready + s, ready[s]);
+                    ready[s] ^= 1;
+                    if (!fine) break;
+                    tc_after_sync();
+                    const uint64_t b = v_desc + (uint32_t)(vs * (L::TILE >> 4));
+#pragma unroll
+                    for (int kk = 0; kk < PT / 16; kk++)
+                        tc_mma_f16_ts(tmem + 2 * PT + s * HD, tmem + s * PT + kk * 8, b + kk * (2048 >> 4), idesc_o, j > 0 || kk > 0, lead);
+                    if (s == 1 || j >= x.tiles1) tc_commit(empty + vs, lead);
+                    if (j + 1 < tiles) {
+                        if (!keys) fine = wait(full + slot, parity);
+                        if (!fine) break;
+                        keys = true;
+                        logits(s);
+                    } else {
+                        tc_commit(o_done + s, lead);
                     }
-                    if (fine && j + 1 < x.n) tc_commit(empty + ks);
-                    if (fine && j + 2 == x.n) tc_commit(q_free);  // the queries have been used for the last time
                 }
+                if (fine && more) tc_commit(empty + slot, lead);
+                if (fine && j + 2 == x.n) tc_commit(q_free, lead);  // the queries have been used for the last time
             }
-            it += 2 * x.n;
-            nu++;
-            fine = __shfl_sync(0xffffffffu, (int)fine, 0);
+            next();
         }
-    } else if (warp == CHECKER) {
+    } else if (warp == CLEARER) {
         if (blockIdx.x == 0) {
             int a, b, c, d;
             for (int s = lane; s < p.nseq; s += 32)
@@ -323,15 +330,13 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (lane == 0) mbar_arrive(full + slot);
         }
     } else {
-        // ---- soft-max: two threads per row, of 64 logits (and half of the result's columns) each
-        const int s = warp >> 3, half = (warp >> 2) & 1, row = (warp & 3) * 32 + lane;
+        // ---- soft-max: thread = row
+        const int s = warp >> 2, row = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;
-        const uint32_t s_at = tmem + s * PT + half * 64 + lanes, p_at = tmem + s * PT + half * 32 + lanes, o_at = tmem + 2 * PT + s * HD + half * (HD / 2) + lanes;
-        float* pair = reinterpret_cast<float*>(smem + L::PAIR) + s * 2 * PT;  // what the two threads of a row tell each other: maxima, sums
-        const int meet = 1 + s * 4 + (warp & 3);                               // their warps' barrier
+        const uint32_t s_at = tmem + s * PT + lanes, o_at = tmem + 2 * PT + s * HD + lanes;
         const float c = fmaxf(fabsf(p.scale) * 1.4426950408889634f, 1e-30f);  // not 0: a masked logit stays below all others
         const bool flip = p.scale < 0.0f;
-        int nt = 0, nu = 0;
+        uint32_t nt = 0, nu = 0;  // parities of the next logits and results
         for (int r = 0;; r++) {
             const int64_t u = unit_of_round(r);
             // The unit is looked up here and again for the results: what describes it does not stay in registers.
@@ -339,67 +344,69 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (!x.find(p, f, u, units, span, two_heads)) break;
             const int mine = s ? x.tiles1 : x.tiles0;
             const int last = min(x.first + (two_heads ? 0 : s * PT) + row + x.nk - x.nq, x.nk - 1);  // the last key that this row sees
-            const int whole = max(0, x.first + x.nk - x.nq + 1) / PT;  // key tiles that every query sees whole
-            float top = -INFINITY, l = 0.0f;  // what the probabilities refer to; the sum of this thread's
-            for (int j = 0; j < mine; j++, nt++) {
-                fine = fine && __all_sync(0xffffffffu, mbar_try_bounded(s_full + s, nt & 1));  // both warps of a row go through all tiles
+            const int whole = max(0, x.first + x.nk - x.nq + 1) / PT;                               // key tiles that every query sees whole
+            float top = -INFINITY, l = 0.0f;  // what the probabilities refer to, their sum
+            for (int j = 0; j < mine; j++, nt ^= 1) {
+                fine = fine && __all_sync(0xffffffffu, mbar_try_bounded(s_full + s, nt));
                 tc_after_sync();
-                float y[64];
-                tc_ld32(s_at, reinterpret_cast<uint32_t*>(y));
-                tc_ld32(s_at + 32, reinterpret_cast<uint32_t*>(y) + 32);
-                tc_wait_ld(reinterpret_cast<uint32_t*>(y));
-                tc_wait_ld(reinterpret_cast<uint32_t*>(y) + 32);
-                if (flip) {
+                const bool masked = j >= whole || flip;
+                const int see = last - j * PT;
+                // 32 logits at a time, the next ones on their way.  Behind the first tile the maximum that probabilities refer
+                // to hardly ever moves, so they are formed with the one there is while the tile's own is found; should it have
+                // to move after all (and in the first tile), the tile is gone through again.
+                float m0, m1;
+                uint32_t pk[PT / 2];  // probabilities, pairs of F16
+                float sum;
+                for (int again = j == 0 ? 0 : 1;; again++) {
+                    const float shift = top == -INFINITY ? 0.0f : -top * c;
+                    const uint64_t cc = f2_pack(c, c), sh = f2_pack(shift, shift);
+                    uint64_t sum2 = 0;
+                    m0 = top, m1 = top;
+                    float y[2][32];
+                    tc_ld32(s_at, reinterpret_cast<uint32_t*>(y[0]));
 #pragma unroll
-                    for (int e = 0; e < 64; e++) y[e] = -y[e];
-                }
-                if (j >= whole) {
-                    const int see = last - j * PT - half * 64;
+                    for (int i = 0; i < PT / 32; i++) {
+                        float* z = y[i & 1];
+                        tc_wait_ld(reinterpret_cast<uint32_t*>(z));
+                        if (i + 1 < PT / 32) tc_ld32(s_at + (i + 1) * 32, reinterpret_cast<uint32_t*>(y[(i + 1) & 1]));
+                        if (masked) {
 #pragma unroll
-                    for (int e = 0; e < 64; e++) y[e] = e <= see ? y[e] : -INFINITY;
-                }
-                float m0 = top, m1 = -INFINITY;
+                            for (int e = 0; e < 32; e++) z[e] = j < whole || 32 * i + e <= see ? (flip ? -z[e] : z[e]) : -INFINITY;
+                        }
 #pragma unroll
-                for (int e = 0; e < 64; e += 4) m0 = max3(m0, y[e], y[e + 1]), m1 = max3(m1, y[e + 2], y[e + 3]);
-                m0 = max3(m0, m1, m1);
-                pair[half * PT + row] = m0;
-                // both halves' logits have been read when this is passed, so that the probabilities may be written over them
-                asm volatile("bar.sync %0, 64;" ::"r"(meet) : "memory");
-                const float m2 = pair[(half ^ 1) * PT + row];
-                m0 = max3(m0, m2, m2);
-                const bool raise = (m0 - top) * c > 8.0f || m0 != m0;  // also the first maximum of a row
-                if (__any_sync(0xffffffffu, raise)) {
+                        for (int e = 0; e < 32; e += 4) m0 = max3(m0, z[e], z[e + 1]), m1 = max3(m1, z[e + 2], z[e + 3]);
+                        if (again) {
+#pragma unroll
+                            for (int e = 0; e < 16; e++) {
+                                const uint64_t w = f2_fma(f2_pack(z[2 * e], z[2 * e + 1]), cc, sh);
+                                const float p0 = ex2(f2_low(w)), p1 = ex2(f2_high(w));
+                                sum2 = f2_add(sum2, f2_pack(p0, p1));
+                                asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(pk[16 * i + e]) : "f"(p1), "f"(p0));
+                            }
+                        }
+                    }
+                    sum = f2_low(sum2) + f2_high(sum2);
+                    m0 = max3(m0, m1, m1);
+                    const bool raise = (m0 - top) * c > 8.0f || (m0 != m0 && top == top);  // also the first maximum of a row
+                    if (again && !__any_sync(0xffffffffu, raise)) break;
                     const float to = raise ? m0 : top, keep = raise ? ex2((top - to) * c) : 1.0f;
                     top = to;
                     l *= keep;
                     if (j > 0) {
 #pragma unroll
                         for (int i = 0; i < HD / 32; i++) {
-                            uint32_t o[16];
-                            tc_ld16(o_at + i * 16, o);
-                            tc_wait_ld16(o);
+                            uint32_t o[32];
+                            tc_ld32(o_at + i * 32, o);
+                            tc_wait_ld(o);
 #pragma unroll
-                            for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-                            tc_st16(o_at + i * 16, o);
+                            for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                            tc_st32(o_at + i * 32, o);
                         }
                     }
                 }
-                const float shift = top == -INFINITY ? 0.0f : -top * c;
-                const uint64_t cc = f2_pack(c, c), sh = f2_pack(shift, shift);
-                uint64_t sum = 0;
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    uint32_t pk[16];
-#pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const uint64_t z = f2_fma(f2_pack(y[32 * i + 2 * e], y[32 * i + 2 * e + 1]), cc, sh);
-                        const float p0 = ex2(f2_low(z)), p1 = ex2(f2_high(z));
-                        sum = f2_add(sum, f2_pack(p0, p1));
-                        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(pk[e]) : "f"(p1), "f"(p0));
-                    }
-                    tc_st16(p_at + i * 16, pk);
-                }
-                l += f2_low(sum) + f2_high(sum);
+                tc_st32(s_at, pk);
+                tc_st32(s_at + 32, pk + 32);
+                l += sum;
                 tc_wait_st();
                 tc_before_sync();
                 __syncwarp();
@@ -409,50 +416,45 @@ __global__ void __launch_bounds__(THREADS, 1)
             f.start(p, span);
             x.find(p, f, u, units, span, two_heads);
             const int at = x.first + (two_heads ? 0 : s * PT) + row;
-            asm volatile("bar.sync %0, 64;" ::"r"(meet) : "memory");  // the other has read the last maximum
-            pair[half * PT + row] = l;
-            asm volatile("bar.sync %0, 64;" ::"r"(meet) : "memory");
-            l += pair[(half ^ 1) * PT + row];
-            asm volatile("bar.sync %0, 64;" ::"r"(meet) : "memory");  // and now the sum
             if (mine > 0) {
-                fine = fine && __all_sync(0xffffffffu, mbar_try_bounded(o_done + s, nu & 1));
-                nu++;
+                fine = fine && __all_sync(0xffffffffu, mbar_try_bounded(o_done + s, nu));
+                nu ^= 1;
             }
             tc_after_sync();
             const bool none = top == -INFINITY, live = fine && at < x.nq;  // no key, or none that counts
             const float inv = none ? 0.0f : 1.0f / l;
             const int head = two_heads ? x.head0 + s : x.head0;
             T* out = reinterpret_cast<T*>(p.out) + (int64_t)head * p.o_head + (int64_t)(x.q0 + at - row) * p.o_tok;  // row 0's
-            T* to = out + (int64_t)row * p.o_tok + half * (HD / 2);
+            T* to = out + (int64_t)row * p.o_tok;
             uint32_t odd = 0;  // sign bit: a result's exponent is all ones
 #pragma unroll
             for (int i = 0; i < HD / 32; i++) {
-                uint32_t o[16];
-                tc_ld16(o_at + i * 16, o);
-                tc_wait_ld16(o);
+                uint32_t o[32];
+                tc_ld32(o_at + i * 32, o);
+                tc_wait_ld(o);
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
+                for (int e = 0; e < 32; e++) {
                     o[e] = none ? 0u : __float_as_uint(__uint_as_float(o[e]) * inv);
                     odd |= (o[e] & 0x7f800000u) + 0x00800000u;
                 }
                 if (!live) continue;
                 if constexpr (sizeof(T) == 4) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) reinterpret_cast<uint4*>(to)[i * 4 + e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                    for (int e = 0; e < 8; e++) reinterpret_cast<uint4*>(to)[i * 8 + e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
                 } else {
-                    uint32_t h[8];
+                    uint32_t h[16];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h[e]) : "f"(__uint_as_float(o[2 * e + 1])), "f"(__uint_as_float(o[2 * e])));
+                    for (int e = 0; e < 16; e++) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h[e]) : "f"(__uint_as_float(o[2 * e + 1])), "f"(__uint_as_float(o[2 * e])));
 #pragma unroll
-                    for (int e = 0; e < 2; e++) reinterpret_cast<uint4*>(to)[i * 2 + e] = make_uint4(h[4 * e], h[4 * e + 1], h[4 * e + 2], h[4 * e + 3]);
+                    for (int e = 0; e < 4; e++) reinterpret_cast<uint4*>(to)[i * 4 + e] = make_uint4(h[4 * e], h[4 * e + 1], h[4 * e + 2], h[4 * e + 3]);
                 }
             }
             tc_before_sync();
-            // this warp's half rows by the plain loop, where one of them is not finite
+            // this warp's rows by the plain loop, where a result is not finite
             if (__any_sync(0xffffffffu, live && (odd >> 31))) {
                 for (int w = 0; w < 32; w++) {
                     const int i = at - lane + w, key = i + x.nk - x.nq + 1;
-                    if (i < x.nq) prompt_row<HD, T>(p.q, p.k, p.v, x.q0 + i, x.k0, key, head, x.kh, p.scale, half, out + (int64_t)(row - lane + w) * p.o_tok);
+                    if (i < x.nq) prompt_row<HD, T>(p.q, p.k, p.v, x.q0 + i, x.k0, key, head, x.kh, p.scale, out + (int64_t)(row - lane + w) * p.o_tok);
                 }
             }
         }
