@@ -17,7 +17,7 @@ import ctypes as C
 
 from ._lib import GaloisCacheQ8, lib
 from .op import _gpu_ctx, _want
-from .tensor import BLCK_SIZE, TYPE_SIZE, Device, GError, GGmlType, Tensor, _check
+from .tensor import Device, GError, GGmlType, Tensor, _check
 
 BLOCK = 32  # rows of a head that share a scale
 
@@ -148,16 +148,18 @@ def galois_cache_attention(q: Tensor, cache: CacheQ8, lens: Tensor, dst: Tensor,
     galois_cache_attention_workspace bytes (any dtype, contents irrelevant; one for each call that may run at the
     same time).  With ``weights`` and ``weights_out`` (F32 {ctx, kv_heads, seqs}; they may be the same tensor) each row's
     probabilities, summed over the heads of its group, are added to its weight."""
-    given = [t for t in (weights, weights_out) if t is not None]
-    ctx = _ctx_of(cache.k, q, lens, dst, workspace, *given)
-    for t in (q, dst, *given):
+    if weights is None and weights_out is None:
+        f32 = (q, dst)
+    else:
+        f32 = tuple(t for t in (q, dst, weights, weights_out) if t is not None)
+    ctx = _ctx_of(cache.k, lens, workspace, *f32)
+    for t in f32:
         if t.dtype is not _F32:
             _want(t, _F32, "galois_cache_attention")
     _ints(lens, cache.seqs, "galois_cache_attention lens")
-    kind, d = workspace.dtype, workspace._dim
-    if not d.ggml_is_contiguous(BLCK_SIZE[kind]):
+    size = workspace.room()
+    if size < 0:
         raise GError("galois_cache_attention: the workspace must be contiguous")
-    size = d.elem_count() // BLCK_SIZE[kind] * TYPE_SIZE[kind]
     w = (None, None) if weights is None else (weights.data_ptr(), weights.c_dim())
     wo = (None, None) if weights_out is None else (weights_out.data_ptr(), weights_out.c_dim())
     rc = lib.galois_b200_cache_attention_f32(ctx, q.data_ptr(), q.c_dim(), cache._ref, lens.data_ptr(), dst.data_ptr(), dst.c_dim(), scale, *w, *wo, workspace.data_ptr(), size)
@@ -171,8 +173,10 @@ def galois_cache_evict(cache: CacheQ8, lens: Tensor, weights: Tensor, recent: in
     rows, ``out_weights`` their weights, ``out_lens`` the new lengths; what lies behind a new length is left as it was."""
     ctx = _ctx_of(cache.k, lens, weights, out.k, out_lens, out_weights, index)
     for t in (weights, out_weights):
-        _want(t, GGmlType.F32, "galois_cache_evict")
-    _want(index, GGmlType.I32, "galois_cache_evict index")
+        if t.dtype is not _F32:
+            _want(t, _F32, "galois_cache_evict")
+    if index.dtype is not _I32:
+        _want(index, _I32, "galois_cache_evict index")
     _ints(lens, cache.seqs, "galois_cache_evict lens")
     _ints(out_lens, cache.seqs, "galois_cache_evict out_lens")
     rc = lib.galois_b200_cache_evict(ctx, cache._ref, lens.data_ptr(), weights.data_ptr(), weights.c_dim(), recent, out._ref, out_lens.data_ptr(), out_weights.data_ptr(),

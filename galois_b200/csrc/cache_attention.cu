@@ -27,12 +27,12 @@ namespace {
 //    fragments are taken as a lane's 16-byte loads give them: of the keys, lane (g, t) has numbers 16 t.. of one row; of
 //    the values, CW numbers of four rows, whose bytes are paired by permutes.  Which row and which chunk g and t stand
 //    for is chosen so that the eight lanes of a load's phase meet no bank of the swizzled tile twice.
-constexpr int WARPS = 12;
+constexpr int WARPS = 8;
 constexpr int BLK = GB_CACHE_BLOCK;
 template <int HD>
 struct ring {
     static constexpr int HALF = BLK * HD;    // bytes of a block's keys (or values)
-    static constexpr int DEPTH = HD == 128 ? 2 : 4;   // tiles of keys, and as many of values
+    static constexpr int DEPTH = HD == 128 ? 3 : 6;   // tiles of keys, and as many of values
     static constexpr int BARS = 1024 + WARPS * 2 * DEPTH * HALF;  // offset of the barriers; 1024 to align the tiles
     static constexpr int TOTAL = BARS + WARPS * 2 * DEPTH * 8;
 };
@@ -110,22 +110,26 @@ __device__ __forceinline__ int64_t count_blocks(const int32_t* __restrict__ lens
     return c * per;
 }
 
-// A place in the list: block `blk` of `blocks` of pair `inner` of sequence `seq`.
-struct cursor {
-    int seq, inner, blk, blocks, len;
-    __device__ __forceinline__ void next_seq(const int32_t* __restrict__ lens, int nseq, int ctx) {
-        do {
-            seq++;
-            len = seq < nseq ? checked_len(lens[seq], ctx) : 1;
-        } while (len == 0);
-        blocks = (len + BLK - 1) / BLK;
-    }
-    __device__ __forceinline__ void advance(const int32_t* __restrict__ lens, int nseq, int ctx, int per) {
-        if (++blk < blocks) return;
+// A place in the list: block `blk` of a pair, with `left` rows from its first to the end.
+struct place {
+    int seq, kh, tile, blk, left, len;
+    // true where a new pair begins
+    __device__ __forceinline__ bool advance(const int32_t* __restrict__ lens, const gb_cache_view& c, int tiles) {
+        blk++, left -= BLK;
+        if (left > 0) return false;
         blk = 0;
-        if (++inner < per) return;
-        inner = 0;
-        next_seq(lens, nseq, ctx);
+        if (++tile == tiles) {
+            tile = 0;
+            if (++kh == c.kv_heads) {
+                kh = 0;
+                do {
+                    seq++;
+                    len = seq < c.seqs ? checked_len(lens[seq], c.ctx) : 1;
+                } while (len == 0);
+            }
+        }
+        left = len;
+        return true;
     }
 };
 
@@ -166,9 +170,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
             if (p.lens[i] < 0 || p.lens[i] > c.ctx) *p.status = GALOIS_B200_E_BADARG;
     const int w = warp * (int)gridDim.x + (int)blockIdx.x;  // parts of neighbours lie on different SMs
     if (w >= D.warps) return;
-    const int64_t b0 = D.begin(w), b1 = D.begin(w + 1);
+    const int64_t b0 = D.begin(w);
+    const int count = (int)(D.begin(w + 1) - b0);
     // the place of block b0
-    cursor at{-1, 0, 0, 0, 0};
+    place at{};
     {
         int64_t before = 0;
         for (int s0 = 0;; s0 += 32) {
@@ -185,9 +190,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
                 const int64_t off = b0 - before - (__shfl_sync(0xffffffffu, upto, l) - __shfl_sync(0xffffffffu, mine, l));
                 at.seq = s0 + l;
                 at.len = __shfl_sync(0xffffffffu, n, l);
-                at.blocks = (at.len + BLK - 1) / BLK;
-                at.inner = (int)(off / at.blocks);
-                at.blk = (int)(off % at.blocks);
+                const int blocks = (at.len + BLK - 1) / BLK, inner = (int)(off / blocks);
+                at.blk = (int)(off % blocks);
+                at.left = at.len - at.blk * BLK;
+                at.kh = inner / p.tiles, at.tile = inner % p.tiles;
                 break;
             }
             before += __shfl_sync(0xffffffffu, upto, 31);
@@ -195,33 +201,32 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     }
     const uint32_t base = ((smem_u32(smem) + 1023u) & ~1023u) + (uint32_t)(warp * 2 * DEPTH * ring<HD>::HALF);
     // Keys are wanted one block earlier than values: the place of the newest keys is kept for the values' next copy.
-    cursor ahead = at;
-    int last_blk = 0, last_kh = 0, last_seq = 0;
-    int64_t fetched = b0;  // blocks whose keys have been asked for
-    // the scales of blocks b.., in the ring's order
+    place ahead = at;
+    int last_row = 0, last_kh = 0, last_seq = 0, to_fetch = count;  // blocks whose keys have not been asked for
+    int64_t scale_at = ahead.kh * c.s_head + ahead.seq * c.s_seq;
+    // the scales of the blocks from the current one on, in the ring's order
     float2 scales[DEPTH + 1];
     auto fetch_keys = [&](int slot) -> float2 {
-        last_blk = ahead.blk, last_kh = ahead.inner / p.tiles, last_seq = ahead.seq;
-        const int64_t sat = last_kh * c.s_head + last_seq * c.s_seq + last_blk;
-        const float2 sc = make_float2(__ldg(c.ks + sat), __ldg(c.vs + sat));
+        last_row = ahead.blk * BLK, last_kh = ahead.kh, last_seq = ahead.seq;
+        const float2 sc = make_float2(c.ks[scale_at + ahead.blk], c.vs[scale_at + ahead.blk]);
         if (lane == 0) {
             mbar_expect_tx(bars + slot, ring<HD>::HALF);
-            tma_load_4d(base + (uint32_t)(slot * ring<HD>::HALF), &k_map, 0, last_blk * BLK, last_kh, last_seq, bars + slot);
+            tma_load_4d(base + (uint32_t)(slot * ring<HD>::HALF), &k_map, 0, last_row, last_kh, last_seq, bars + slot);
         }
-        ahead.advance(p.lens, c.seqs, c.ctx, per);
-        fetched++;
+        if (ahead.advance(p.lens, c, p.tiles)) scale_at = ahead.kh * c.s_head + ahead.seq * c.s_seq;
+        to_fetch--;
         return sc;
     };
     auto fetch_values = [&](int slot) {
         if (lane == 0) {
             mbar_expect_tx(bars + DEPTH + slot, ring<HD>::HALF);
-            tma_load_4d(base + (uint32_t)((DEPTH + slot) * ring<HD>::HALF), &v_map, 0, last_blk * BLK, last_kh, last_seq, bars + DEPTH + slot);
+            tma_load_4d(base + (uint32_t)((DEPTH + slot) * ring<HD>::HALF), &v_map, 0, last_row, last_kh, last_seq, bars + DEPTH + slot);
         }
     };
 #pragma unroll
     for (int i = 0; i < DEPTH; i++) {
         scales[i] = make_float2(0.f, 0.f);
-        if (fetched < b1) scales[i] = fetch_keys(i), fetch_values(i);
+        if (to_fetch > 0) scales[i] = fetch_keys(i), fetch_values(i);
     }
     scales[DEPTH] = make_float2(0.f, 0.f);
     uint32_t phases = 0;  // bit i: parity that barrier i completes next
@@ -233,16 +238,20 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
 
     uint32_t qa[KS][4];
     float factor = 0.0f;
+    bool live = false;       // this lane's head exists
+    float* scores = nullptr;  // its logits' row, where they are wanted
     // The query of the pair at `at`: lane (g, t) holds numbers 16 (t + 4 i) + 4 j.. of head g, times the power of two that
     // brings the largest to 2^7..2^8, as two F16 each.
     auto load_query = [&]() {
-        const int head0 = at.inner / p.tiles * p.group + (at.inner % p.tiles) * 8, live = min(8, p.group - (at.inner % p.tiles) * 8);
+        const int head = at.kh * p.group + at.tile * 8 + g;
+        live = g < p.group - at.tile * 8;
         float4 f[KS];
         float top = 0.0f;
-        const float* qh = p.q + (int64_t)(head0 + g) * p.q_head + (int64_t)at.seq * p.q_seq;
+        const float* qh = p.q + (int64_t)head * p.q_head + (int64_t)at.seq * p.q_seq;
+        scores = live && p.scores ? p.scores + ((int64_t)at.seq * heads + head) * c.ctx : nullptr;
 #pragma unroll
         for (int i = 0; i < KS; i++) {
-            f[i] = g < live ? *reinterpret_cast<const float4*>(qh + 16 * (t + 4 * (i / 4)) + 4 * (i % 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            f[i] = live ? *reinterpret_cast<const float4*>(qh + 16 * (t + 4 * (i / 4)) + 4 * (i % 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
             top = fmaxf(top, fmaxf(fmaxf(fabsf(f[i].x), fabsf(f[i].y)), fmaxf(fabsf(f[i].z), fabsf(f[i].w))));
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -294,31 +303,27 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     bool fine = wait(0);
     logits(0, scales[0].x, x);
     __syncwarp();
-    bool more = fetched < b1;  // the block behind the ring exists: its keys now, its values when block b's are used
+    bool more = to_fetch > 0;  // the block behind the ring exists: its keys now, its values when this block's are used
     if (more) scales[DEPTH] = fetch_keys(0);
-    for (int64_t b = b0; b < b1 && fine; b++) {
+    for (int todo = count; todo > 0 && fine; todo--) {
         const int next = slot + 1 == DEPTH ? 0 : slot + 1;
-        if (b + 1 < b1) fine = wait(next);
+        if (todo > 1) fine = wait(next);
         logits(next, scales[1].x, xn);  // formed again below if a new pair begins there; of no use behind the last block
         fine = fine && wait(DEPTH + slot);
         const uint32_t vs = base + (uint32_t)((DEPTH + slot) * ring<HD>::HALF);
-        const int left = at.len - at.blk * BLK;
-        if (left < BLK) {
+        if (at.left < BLK) {
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                if (row_of<HD>(j, 2 * t) >= left) x[j][0] = -INFINITY;
-                if (row_of<HD>(j, 2 * t + 1) >= left) x[j][1] = -INFINITY;
+                if (row_of<HD>(j, 2 * t) >= at.left) x[j][0] = -INFINITY;
+                if (row_of<HD>(j, 2 * t + 1) >= at.left) x[j][1] = -INFINITY;
             }
         }
-        if (p.scores) {
-            const int head0 = at.inner / p.tiles * p.group + (at.inner % p.tiles) * 8, live = min(8, p.group - (at.inner % p.tiles) * 8);
-            if (g < live) {
-                float* to = p.scores + ((int64_t)at.seq * heads + head0 + g) * c.ctx + at.blk * BLK;
+        if (scores) {
+            float* to = scores + at.blk * BLK;
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    if (row_of<HD>(j, 2 * t) < left) to[row_of<HD>(j, 2 * t)] = x[j][0];
-                    if (row_of<HD>(j, 2 * t + 1) < left) to[row_of<HD>(j, 2 * t + 1)] = x[j][1];
-                }
+            for (int j = 0; j < 4; j++) {
+                if (row_of<HD>(j, 2 * t) < at.left) to[row_of<HD>(j, 2 * t)] = x[j][0];
+                if (row_of<HD>(j, 2 * t + 1) < at.left) to[row_of<HD>(j, 2 * t + 1)] = x[j][1];
             }
         }
         float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1])), fmaxf(fmaxf(x[2][0], x[2][1]), fmaxf(x[3][0], x[3][1])));
@@ -384,14 +389,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
         if (more) fetch_values(slot);
 #pragma unroll
         for (int i = 0; i < DEPTH; i++) scales[i] = scales[i + 1];
-        const int64_t item = (int64_t)at.seq * per + at.inner;
-        const int live = min(8, p.group - (at.inner % p.tiles) * 8);
-        at.advance(p.lens, c.seqs, c.ctx, per);
+        const int64_t item = (int64_t)at.seq * per + at.kh * p.tiles + at.tile;
         slot = next;
-        if (at.blk == 0 || b + 1 == b1) {  // this warp's piece of the pair
+        if (at.advance(p.lens, c, p.tiles) || todo == 1) {  // this warp's piece of the pair
             l += __shfl_xor_sync(0xffffffffu, l, 1);
             l += __shfl_xor_sync(0xffffffffu, l, 2);
-            if (g < live) {
+            if (live) {
                 const int64_t row = (w + item) * p.rows + g;
                 if (t == 0) *reinterpret_cast<float2*>(p.stats + 2 * row) = make_float2(m, l);
                 // column 2 t of an n-tile stands for chunk t of a 128-byte row (column 2 t + 1 for chunk t + 4), or bytes 16 t (+ 8) of a 64-byte one
@@ -406,13 +409,13 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
 #pragma unroll
             for (int i = 0; i < NW * 4; i++) o[i] = 0;
             m = -INFINITY, l = 0.0f, vtop = 0.0f, vinv = 0.0f;
-            if (b + 1 < b1) {
+            if (todo > 1) {
                 load_query();
                 logits(next, scales[0].x, xn);
             }
         }
         __syncwarp();
-        more = fetched < b1;
+        more = to_fetch > 0;
         if (more) scales[DEPTH] = fetch_keys(next);
 #pragma unroll
         for (int j = 0; j < 4; j++) x[j][0] = xn[j][0], x[j][1] = xn[j][1];
@@ -454,22 +457,44 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const int32_t* __restri
         const int64_t first = before * per + (int64_t)inner * blocks;
         const int w0 = D.owner(first), n = D.owner(first + blocks - 1) - w0 + 1;
         const int64_t row0 = (w0 + (int64_t)s * per + inner) * rows + r;
+        // a lane holds what the pieces lane, lane + 32, .. say of themselves; the first 128 stay in registers
+        float2 st[4];
         float m = -INFINITY;
-        for (int i = lane; i < n; i += 32) m = fmaxf(m, stats[2 * (row0 + (int64_t)i * rows)]);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            st[i] = make_float2(-INFINITY, 0.0f);
+            if (lane + 32 * i < n) st[i] = *reinterpret_cast<const float2*>(stats + 2 * (row0 + (int64_t)(lane + 32 * i) * rows));
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) m = fmaxf(m, st[i].x);
+        for (int i = lane + 128; i < n; i += 32) m = fmaxf(m, stats[2 * (row0 + (int64_t)i * rows)]);
         m = gb_warp_max(m);
         use = m == -INFINITY ? 0.0f : m;
-        for (int i = lane; i < n; i += 32) {
-            const float2 st = *reinterpret_cast<const float2*>(stats + 2 * (row0 + (int64_t)i * rows));
-            l += st.y * ex2(st.x - use);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            st[i].x = ex2(st[i].x - use);  // the piece's share
+            l += st[i].y * st[i].x;
+        }
+        for (int i = lane + 128; i < n; i += 32) {
+            const float2 s2 = *reinterpret_cast<const float2*>(stats + 2 * (row0 + (int64_t)i * rows));
+            l += s2.y * ex2(s2.x - use);
         }
         l = gb_warp_sum(l);
-#pragma unroll 4
-        for (int i = wr; i < n; i += W) {
-            const int64_t row = row0 + (int64_t)i * rows;
-            const float f = ex2(stats[2 * row] - use);
-            const float* a = acc + row * HD + lane * E;
+        const float* a = acc + row0 * HD + lane * E;
 #pragma unroll
-            for (int e = 0; e < E; e++) x[e] = fmaf(a[e], f, x[e]);
+        for (int k = 0; k < 4; k++) {
+            const int end = min(n, 32 * (k + 1));
+#pragma unroll 8
+            for (int i = 32 * k + wr; i < end; i += W) {
+                const float f = __shfl_sync(0xffffffffu, st[k].x, i & 31);
+#pragma unroll
+                for (int e = 0; e < E; e++) x[e] = fmaf(a[(int64_t)i * rows * HD + e], f, x[e]);
+            }
+        }
+        for (int i = 128 + wr; i < n; i += W) {
+            const float f = ex2(stats[2 * (row0 + (int64_t)i * rows)] - use);
+#pragma unroll
+            for (int e = 0; e < E; e++) x[e] = fmaf(a[(int64_t)i * rows * HD + e], f, x[e]);
         }
     }
     if constexpr (W > 1) {

@@ -194,7 +194,7 @@ class Tensor:
         self.storage = storage
         self.device = device
         self.offset = offset  # in elements (blocks for Q4_0) from the start of `storage`
-        self._c_dim = None
+        self._c_dim = self._room = None
 
     # ---- constructors ------------------------------------------------
     @staticmethod
@@ -259,6 +259,13 @@ class Tensor:
             self._c_dim = C.byref(self._dim.c_struct())
         return self._c_dim
 
+    def room(self) -> int:
+        """Bytes of a contiguous tensor, -1 for any other; found once, like ``c_dim``."""
+        if self._room is None:
+            per = BLCK_SIZE[self.dtype]
+            self._room = self._dim.elem_count() // per * TYPE_SIZE[self.dtype] if self._dim.ggml_is_contiguous(per) else -1
+        return self._room
+
     def shape(self):
         return self._dim.shape[: self._dim.n_dims]
 
@@ -267,9 +274,10 @@ class Tensor:
         return self.device.is_gpu
 
     def data_ptr(self) -> int:
-        if not self.is_gpu:
+        if self.device.gpu is None:
             raise GError("data_ptr: CPU tensor")
-        return self.storage.data_ptr() + self.offset * TYPE_SIZE[self.dtype]
+        at = self.storage.data_ptr()
+        return at + self.offset * TYPE_SIZE[self.dtype] if self.offset else at
 
     def view(self, shape, stride, offset: int = 0) -> "Tensor":
         """A strided window on the same storage (shape/stride in ggml order, stride and
