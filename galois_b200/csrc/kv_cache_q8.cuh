@@ -33,6 +33,7 @@ static inline bool gb_overlap(const void* a, size_t an, const void* b, size_t bn
 }
 // No two elements at one address: sorted by stride, each dimension steps over all of the smaller ones.
 static inline bool gb_injective(const galois_dim* d) {
+    if (gb_span(d, 1) == 0) return true;
     int64_t span = 1;
     bool used[4] = {false, false, false, false};
     for (int k = 0; k < 4; k++) {

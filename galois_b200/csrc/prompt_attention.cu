@@ -8,19 +8,19 @@
 // 4 head_dim flops a pair of query and key against 4 bytes a token: bound by the tensor cores, and next to them by the
 // exponentials (16 a cycle and SM against 32 pairs a cycle that the tensor cores get through).
 //
-//   warps 0-7, 8-15  soft-max of query tile 0, 1 (128 rows each, two threads per row: 64 logits each)
-//   warp 16          loader: TMA copies of the query tiles, then keys and values, 128 rows at a time, through a ring of slots
-//   warp 17          issues the tensor-core products and owns the tensor memory
-//   warp 18          clears what lies behind a sequence's end in its last tile of values
+//   warps 0-3, 4-7  soft-max of query tile 0, 1 (128 rows each, a thread per row)
+//   warp 8          loader: TMA copies of the query tiles, then keys and values, 64 rows at a time, through a ring of slots
+//   warp 9          issues the tensor-core products and owns the tensor memory
+//   warp 10         clears what lies behind a sequence's end in its last tile of values
 //
 // One CTA per SM goes through units of two query tiles (those that see most keys first), and every role runs ahead on its
 // own: keys of the next unit are loaded, and its first logits formed, while the results of this one are written.  The two
 // query tiles share the keys: two heads of a group over the same tokens where the group is even (their masks agree), else
-// two runs of tokens of one head.  While one tile's logits are in the soft-max, the tensor cores work for the other.  Tensor
-// memory: logits 2 x 128 columns, results 2 x head_dim; the probabilities (F16) overwrite the first half of their logits and
-// are the second product's operand from there.  The running maximum that probabilities refer to is raised only when a row's
-// maximum passes it by 2^8 (F16 holds what that leaves), so that the results in tensor memory are rarely rescaled; the
-// logits' barrier also says that the products before them are done, so the rescaling needs no other.
+// two runs of tokens of one head.  Tensor memory: for each query tile two buffers of logits, 2 x 64 columns, so that the
+// tensor cores form the next logits while the soft-max has these, and the results, head_dim columns; the probabilities (F16)
+// overwrite the first half of their logits and are the second product's operand from there.  The running maximum that
+// probabilities refer to is raised only when a row's maximum passes it by 2^8 (F16 holds what that leaves), so that the
+// results in tensor memory are rarely rescaled.
 //
 // A probability of 0 does not hide a value that is not finite: where a result is not finite, its rows are formed again by
 // the plain loop below, which reads nothing that a query does not see.
@@ -67,14 +67,16 @@ __device__ __noinline__ void prompt_row(const rows16& q, const rows16& k, const 
     }
 }
 
-constexpr int PT = 128;      // rows of a tile of queries, of keys, of values
+constexpr int PT = 128;  // rows of a tile of queries
+constexpr int KT = 64;   // rows of a tile of keys, of values
 constexpr int LOADER = 8, ISSUER = 9, CLEARER = 10;  // warps behind the soft-max's
 constexpr int THREADS = 11 * 32;
 template <int HD>
 struct plan {
-    static constexpr uint32_t TILE = PT * HD * 2, HALF = PT * 128;  // bytes of a tile; of its first 64 columns
-    static constexpr int SLOTS = HD == 128 ? 5 : 12;                // tiles of keys and values in shared memory
-    static constexpr uint32_t Q = 0, KV = 2 * TILE, BARS = KV + SLOTS * TILE, TOTAL = BARS + 320;
+    static constexpr uint32_t Q_TILE = PT * HD * 2, Q_HALF = PT * 128;  // bytes of a tile; of its first 64 columns
+    static constexpr uint32_t TILE = KT * HD * 2, HALF = KT * 128;
+    static constexpr int SLOTS = HD == 128 ? 10 : 20;                   // tiles of keys and values in shared memory
+    static constexpr uint32_t Q = 0, KV = 2 * Q_TILE, BARS = KV + SLOTS * TILE, TOTAL = BARS + 512;
     static_assert(TOTAL <= 227 * 1024, "shared memory");
 };
 struct prompt_args {
@@ -164,10 +166,10 @@ struct prompt_unit {
     }
     __device__ __forceinline__ int tiles(int off) const {
         const int rows = min(PT, nq - first - off);
-        return rows > 0 ? (max(0, first + off + rows + nk - nq) + PT - 1) / PT : 0;
+        return rows > 0 ? (max(0, first + off + rows + nk - nq) + KT - 1) / KT : 0;
     }
     // the last tile of values reaches behind the sequence's end
-    __device__ __forceinline__ bool ragged() const { return n > 0 && n * PT > nk; }
+    __device__ __forceinline__ bool ragged() const { return n > 0 && n * KT > nk; }
 };
 
 template <int HD, typename T>
@@ -178,15 +180,16 @@ __global__ void __launch_bounds__(THREADS, 1)
     constexpr int SLOTS = L::SLOTS;
     extern __shared__ __align__(1024) uint8_t smem[];  // swizzled tiles start at multiples of 1024
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
-    uint64_t *q_full = bars, *q_free = bars + 1, *full = bars + 2, *empty = full + SLOTS, *s_full = empty + SLOTS, *p_ready = s_full + 2, *o_done = p_ready + 2,
-             *v_raw = o_done + 2;
+    uint64_t *q_full = bars, *q_free = bars + 1, *full = bars + 2, *empty = full + SLOTS, *s_full = empty + SLOTS, *p_ready = s_full + 4, *pv_done = p_ready + 4,
+             *v_raw = pv_done + 2;  // s_full, p_ready: [query tile][buffer]
     uint32_t* tmem_at = reinterpret_cast<uint32_t*>(v_raw + 1);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) {
         tma_prefetch_map(&q_map), tma_prefetch_map(&k_map), tma_prefetch_map(&v_map);
         mbar_init(q_full, 1), mbar_init(q_free, 1), mbar_init(v_raw, 1);
         for (int i = 0; i < SLOTS; i++) mbar_init(full + i, 1), mbar_init(empty + i, 1);
-        for (int i = 0; i < 2; i++) mbar_init(s_full + i, 1), mbar_init(p_ready + i, 4), mbar_init(o_done + i, 1);
+        for (int i = 0; i < 4; i++) mbar_init(s_full + i, 1), mbar_init(p_ready + i, 4);
+        for (int i = 0; i < 2; i++) mbar_init(pv_done + i, 1);
         fence_mbarrier_init_cluster();
     }
     if (warp == ISSUER) {
@@ -213,13 +216,16 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (lane == 0) {
                 if (nu > 0) fine = mbar_try_bounded(q_free, (nu - 1) & 1);
                 if (fine) {
-                    mbar_expect_tx(q_full, 2 * L::TILE);
+                    mbar_expect_tx(q_full, 2 * L::Q_TILE);
                     for (int s = 0; s < 2; s++)
                         for (int h = 0; h < HD / 64; h++)
-                            tma_load_3d(smem_u32(smem + L::Q) + s * L::TILE + h * L::HALF, &q_map, 64 * h, x.q0 + x.first + (two_heads ? 0 : s * PT),
+                            tma_load_3d(smem_u32(smem + L::Q) + s * L::Q_TILE + h * L::Q_HALF, &q_map, 64 * h, x.q0 + x.first + (two_heads ? 0 : s * PT),
                                         two_heads ? x.head0 + s : x.head0, q_full);
                 }
+                // in the order of their use: two tiles of keys, then values and the keys after next in turn
                 for (int i = 0; i < 2 * x.n && fine; i++, it++) {
+                    const bool keys = i == 0 || (i == 1 && x.n > 1) || ((i & 1) && (i >> 1) + 1 < x.n);
+                    const int tile = i < 2 ? (keys ? i : 0) : (i & 1) ? (keys ? (i >> 1) + 1 : i >> 1) : (i >> 1) - 1;
                     const int slot = it % SLOTS;
                     if (it >= SLOTS) fine = mbar_try_bounded(empty + slot, (it / SLOTS - 1) & 1);
                     if (!fine) break;
@@ -227,7 +233,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     uint64_t* bar = i == 2 * x.n - 1 && x.ragged() ? v_raw : full + slot;
                     mbar_expect_tx(bar, L::TILE);
                     for (int h = 0; h < HD / 64; h++)
-                        tma_load_3d(smem_u32(smem + L::KV) + slot * L::TILE + h * L::HALF, (i & 1) ? &v_map : &k_map, 64 * h, x.k0 + (i >> 1) * PT, x.kh, bar);
+                        tma_load_3d(smem_u32(smem + L::KV) + slot * L::TILE + h * L::HALF, keys ? &k_map : &v_map, 64 * h, x.k0 + tile * KT, x.kh, bar);
                 }
             }
             nu++;
@@ -243,70 +249,74 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
     } else if (warp == ISSUER) {
         // f32 sums, F16 operands; logits: keys as they are; results: values with the contraction along their rows
-        const uint32_t idesc_s = (1u << 4) | ((uint32_t)(PT >> 3) << 17) | ((uint32_t)(PT >> 4) << 24);
+        const uint32_t idesc_s = (1u << 4) | ((uint32_t)(KT >> 3) << 17) | ((uint32_t)(PT >> 4) << 24);
         const uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(PT >> 4) << 24);
         // The whole warp goes through this, and one thread of it issues (see tc_elect).
         const uint32_t lead = tc_elect();
         const uint64_t q_desc = tc_desc(smem_u32(smem + L::Q), 16, 1024, 128), k_desc = tc_desc(smem_u32(smem + L::KV), 16, 1024, 128),
                        v_desc = tc_desc(smem_u32(smem + L::KV), L::HALF, 1024, 128);
         int slot = 0;
-        uint32_t parity = 0, q_parity = 0;   // of the ring's round, of the next queries
-        uint32_t ready[2] = {0, 0};          // of the next probabilities of each query tile
+        uint32_t parity = 0, q_parity = 0;  // of the ring's round, of the next queries
+        uint32_t ready = 0;                 // bit 2 s + b: of the next probabilities of query tile s in buffer b
         auto next = [&]() {
             if (++slot == SLOTS) slot = 0, parity ^= 1;
         };
         auto wait = [&](uint64_t* bar, uint32_t phase) { return __all_sync(0xffffffffu, mbar_try_bounded(bar, phase)) != 0; };
-        auto logits = [&](int s) {  // of the keys in `slot`
-            const uint64_t a = q_desc + (uint32_t)(s * (L::TILE >> 4)), b = k_desc + (uint32_t)(slot * (L::TILE >> 4));
+        auto logits = [&](int s, int b) {  // of the keys in `slot`, into buffer b
+            const uint64_t q = q_desc + (uint32_t)(s * (L::Q_TILE >> 4)), k = k_desc + (uint32_t)(slot * (L::TILE >> 4));
 #pragma unroll
             for (int kk = 0; kk < HD / 16; kk++) {
-                constexpr uint32_t H = L::HALF >> 4;
-                tc_mma_f16_ss(tmem + s * PT, a + (kk / 4 * H + kk % 4 * 2), b + (kk / 4 * H + kk % 4 * 2), idesc_s, kk > 0, lead);
+                constexpr uint32_t QH = L::Q_HALF >> 4, KH = L::HALF >> 4;
+                tc_mma_f16_ss(tmem + s * PT + b * KT, q + (kk / 4 * QH + kk % 4 * 2), k + (kk / 4 * KH + kk % 4 * 2), idesc_s, kk > 0, lead);
             }
-            tc_commit(s_full + s, lead);
+            tc_commit(s_full + 2 * s + b, lead);
         };
         for (int r = 0; fine && x.find(p, f, unit_of_round(r), units, span, two_heads); r++) {
             if (x.n == 0) continue;
-            fine = wait(q_full, q_parity) && wait(full + slot, parity);
+            fine = wait(q_full, q_parity);
             q_parity ^= 1;
-            if (!fine) break;
-            if (x.tiles0 > 0) logits(0);
-            if (x.tiles1 > 0) logits(1);
-            tc_commit(empty + slot, lead);
-            if (x.n == 1) tc_commit(q_free, lead);
-            for (int j = 0; j < x.n && fine; j++) {
+            for (int b = 0; b < 2 && b < x.n && fine; b++) {
+                fine = wait(full + slot, parity);
+                if (!fine) break;
+                if (x.tiles0 > b) logits(0, b);
+                if (x.tiles1 > b) logits(1, b);
+                tc_commit(empty + slot, lead);
                 next();
-                const int vs = slot;
+            }
+            if (fine && x.n <= 2) tc_commit(q_free, lead);  // the queries have been used for the last time
+            for (int j = 0; j < x.n && fine; j++) {
+                const int vs = slot, b = j & 1;
                 fine = wait(full + vs, parity);
-                const bool more = j + 1 < x.n;
-                if (more) next();
-                bool keys = false;  // the next keys have arrived
+                next();
+                const bool more = j + 2 < x.n;  // the keys after next lie in `slot`
+                bool keys = false;              // they have arrived
 #pragma unroll
                 for (int s = 0; s < 2; s++) {
                     const int tiles = s ? x.tiles1 : x.tiles0;
                     if (j >= tiles || !fine) continue;
-                    fine = wait(p_ready + s, ready[s]);
-                    ready[s] ^= 1;
+                    fine = wait(p_ready + 2 * s + b, (ready >> (2 * s + b)) & 1);
+                    ready ^= 1u << (2 * s + b);
                     if (!fine) break;
                     tc_after_sync();
-                    const uint64_t b = v_desc + (uint32_t)(vs * (L::TILE >> 4));
+                    const uint64_t v = v_desc + (uint32_t)(vs * (L::TILE >> 4));
 #pragma unroll
-                    for (int kk = 0; kk < PT / 16; kk++)
-                        tc_mma_f16_ts(tmem + 2 * PT + s * HD, tmem + s * PT + kk * 8, b + kk * (2048 >> 4), idesc_o, j > 0 || kk > 0, lead);
+                    for (int kk = 0; kk < KT / 16; kk++)
+                        tc_mma_f16_ts(tmem + 2 * PT + s * HD, tmem + s * PT + b * KT + kk * 8, v + kk * (2048 >> 4), idesc_o, j > 0 || kk > 0, lead);
+                    tc_commit(pv_done + s, lead);
                     if (s == 1 || j >= x.tiles1) tc_commit(empty + vs, lead);
-                    if (j + 1 < tiles) {
+                    if (j + 2 < tiles) {
                         if (!keys) fine = wait(full + slot, parity);
                         if (!fine) break;
                         keys = true;
-                        logits(s);
-                    } else {
-                        tc_commit(o_done + s, lead);
+                        logits(s, b);
                     }
                 }
-                if (fine && more) tc_commit(empty + slot, lead);
-                if (fine && j + 2 == x.n) tc_commit(q_free, lead);  // the queries have been used for the last time
+                if (fine && more) {
+                    tc_commit(empty + slot, lead);
+                    next();
+                    if (j + 3 == x.n) tc_commit(q_free, lead);
+                }
             }
-            next();
         }
     } else if (warp == CLEARER) {
         if (blockIdx.x == 0) {
@@ -321,10 +331,10 @@ __global__ void __launch_bounds__(THREADS, 1)
             fine = __all_sync(0xffffffffu, mbar_try_bounded(v_raw, nr & 1));
             nr++;
             if (!fine) break;
-            const int slot = (it - 1) % SLOTS, valid = x.nk - (x.n - 1) * PT;
+            const int slot = (it - 1) % SLOTS, valid = x.nk - (x.n - 1) * KT;
             uint4* v = reinterpret_cast<uint4*>(smem + L::KV + slot * L::TILE);  // [half][row][8 pieces]
             for (int h = 0; h < HD / 64; h++)
-                for (int i = valid * 8 + lane; i < PT * 8; i += 32) v[h * PT * 8 + i] = make_uint4(0, 0, 0, 0);
+                for (int i = valid * 8 + lane; i < KT * 8; i += 32) v[h * KT * 8 + i] = make_uint4(0, 0, 0, 0);
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(full + slot);
@@ -336,7 +346,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const uint32_t s_at = tmem + s * PT + lanes, o_at = tmem + 2 * PT + s * HD + lanes;
         const float c = fmaxf(fabsf(p.scale) * 1.4426950408889634f, 1e-30f);  // not 0: a masked logit stays below all others
         const bool flip = p.scale < 0.0f;
-        uint32_t nt = 0, nu = 0;  // parities of the next logits and results
+        uint32_t nt = 0, done = 0;  // bit b: parity of the next logits in buffer b; key tiles of all units so far
         for (int r = 0;; r++) {
             const int64_t u = unit_of_round(r);
             // The unit is looked up here and again for the results: what describes it does not stay in registers.
@@ -344,55 +354,56 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (!x.find(p, f, u, units, span, two_heads)) break;
             const int mine = s ? x.tiles1 : x.tiles0;
             const int last = min(x.first + (two_heads ? 0 : s * PT) + row + x.nk - x.nq, x.nk - 1);  // the last key that this row sees
-            const int whole = max(0, x.first + x.nk - x.nq + 1) / PT;                               // key tiles that every query sees whole
+            const int whole = max(0, x.first + (two_heads ? 0 : s * PT) + x.nk - x.nq + 1) / KT;    // key tiles that the first row, and so all, see whole
             float top = -INFINITY, l = 0.0f;  // what the probabilities refer to, their sum
-            for (int j = 0; j < mine; j++, nt ^= 1) {
-                fine = fine && __all_sync(0xffffffffu, mbar_try_bounded(s_full + s, nt));
+            for (int j = 0; j < mine; j++) {
+                const uint32_t b = j & 1, b_at = s_at + b * KT;
+                fine = fine && __all_sync(0xffffffffu, mbar_try_bounded(s_full + 2 * s + b, (nt >> b) & 1));
+                nt ^= 1u << b;
                 tc_after_sync();
-                const bool masked = j >= whole || flip;
-                const int see = last - j * PT;
-                // 32 logits at a time, the next ones on their way.  Behind the first tile the maximum that probabilities refer
-                // to hardly ever moves, so they are formed with the one there is while the tile's own is found; should it have
-                // to move after all (and in the first tile), the tile is gone through again.
-                float m0, m1;
-                uint32_t pk[PT / 2];  // probabilities, pairs of F16
-                float sum;
-                for (int again = j == 0 ? 0 : 1;; again++) {
+                float y[KT];
+#pragma unroll
+                for (int i = 0; i < KT / 32; i++) tc_ld32(b_at + i * 32, reinterpret_cast<uint32_t*>(y) + i * 32);
+#pragma unroll
+                for (int i = 0; i < KT / 32; i++) tc_wait_ld(reinterpret_cast<uint32_t*>(y) + i * 32);
+                if (flip) {
+#pragma unroll
+                    for (int e = 0; e < KT; e++) y[e] = -y[e];
+                }
+                if (j >= whole) {
+                    const int see = last - j * KT;
+#pragma unroll
+                    for (int e = 0; e < KT; e++) y[e] = e <= see ? y[e] : -INFINITY;
+                }
+                uint32_t pk[KT / 2];  // probabilities, pairs of F16
+                uint64_t sums[2];
+                auto exponentials = [&]() {
                     const float shift = top == -INFINITY ? 0.0f : -top * c;
                     const uint64_t cc = f2_pack(c, c), sh = f2_pack(shift, shift);
-                    uint64_t sum2 = 0;
-                    m0 = top, m1 = top;
-                    float y[2][32];
-                    tc_ld32(s_at, reinterpret_cast<uint32_t*>(y[0]));
+                    sums[0] = sums[1] = 0;
 #pragma unroll
-                    for (int i = 0; i < PT / 32; i++) {
-                        float* z = y[i & 1];
-                        tc_wait_ld(reinterpret_cast<uint32_t*>(z));
-                        if (i + 1 < PT / 32) tc_ld32(s_at + (i + 1) * 32, reinterpret_cast<uint32_t*>(y[(i + 1) & 1]));
-                        if (masked) {
-#pragma unroll
-                            for (int e = 0; e < 32; e++) z[e] = j < whole || 32 * i + e <= see ? (flip ? -z[e] : z[e]) : -INFINITY;
-                        }
-#pragma unroll
-                        for (int e = 0; e < 32; e += 4) m0 = max3(m0, z[e], z[e + 1]), m1 = max3(m1, z[e + 2], z[e + 3]);
-                        if (again) {
-#pragma unroll
-                            for (int e = 0; e < 16; e++) {
-                                const uint64_t w = f2_fma(f2_pack(z[2 * e], z[2 * e + 1]), cc, sh);
-                                const float p0 = ex2(f2_low(w)), p1 = ex2(f2_high(w));
-                                sum2 = f2_add(sum2, f2_pack(p0, p1));
-                                asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(pk[16 * i + e]) : "f"(p1), "f"(p0));
-                            }
-                        }
+                    for (int e = 0; e < KT / 2; e++) {
+                        const uint64_t w = f2_fma(f2_pack(y[2 * e], y[2 * e + 1]), cc, sh);
+                        const float p0 = ex2(f2_low(w)), p1 = ex2(f2_high(w));
+                        sums[e & 1] = f2_add(sums[e & 1], f2_pack(p0, p1));
+                        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(pk[e]) : "f"(p1), "f"(p0));
                     }
-                    sum = f2_low(sum2) + f2_high(sum2);
-                    m0 = max3(m0, m1, m1);
-                    const bool raise = (m0 - top) * c > 8.0f || (m0 != m0 && top == top);  // also the first maximum of a row
-                    if (again && !__any_sync(0xffffffffu, raise)) break;
-                    const float to = raise ? m0 : top, keep = raise ? ex2((top - to) * c) : 1.0f;
-                    top = to;
+                };
+                float m[4] = {top, top, top, top};
+#pragma unroll
+                for (int e = 0; e < KT; e += 2) m[(e >> 1) & 3] = max3(m[(e >> 1) & 3], y[e], y[e + 1]);
+                const float most = max3(max3(m[0], m[1], m[2]), m[3], m[3]);
+                // Behind the first tile the maximum that probabilities refer to hardly ever moves, so they are formed with the
+                // one there is, beside the search for the tile's own; should it have to move after all, they are formed again.
+                if (j > 0) exponentials();
+                const bool raise = (most - top) * c > 8.0f || (most != most && top == top);  // also the first maximum of a row
+                if (j == 0 || __any_sync(0xffffffffu, raise)) {
+                    const float keep = raise ? ex2((top - most) * c) : 1.0f;
+                    if (raise) top = most;
                     l *= keep;
                     if (j > 0) {
+                        fine = fine && __all_sync(0xffffffffu, mbar_try_bounded(pv_done + s, (done + j - 1) & 1));
+                        tc_after_sync();
 #pragma unroll
                         for (int i = 0; i < HD / 32; i++) {
                             uint32_t o[32];
@@ -403,23 +414,22 @@ __global__ void __launch_bounds__(THREADS, 1)
                             tc_st32(o_at + i * 32, o);
                         }
                     }
+                    exponentials();
                 }
-                tc_st32(s_at, pk);
-                tc_st32(s_at + 32, pk + 32);
-                l += sum;
+                tc_st32(b_at, pk);
+                sums[0] = f2_add(sums[0], sums[1]);
+                l += f2_low(sums[0]) + f2_high(sums[0]);
                 tc_wait_st();
                 tc_before_sync();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(p_ready + s);
+                if (lane == 0) mbar_arrive(p_ready + 2 * s + b);
             }
+            done += mine;
             // ---- results
             f.start(p, span);
             x.find(p, f, u, units, span, two_heads);
             const int at = x.first + (two_heads ? 0 : s * PT) + row;
-            if (mine > 0) {
-                fine = fine && __all_sync(0xffffffffu, mbar_try_bounded(o_done + s, nu));
-                nu ^= 1;
-            }
+            if (mine > 0) fine = fine && __all_sync(0xffffffffu, mbar_try_bounded(pv_done + s, (done - 1) & 1));
             tc_after_sync();
             const bool none = top == -INFINITY, live = fine && at < x.nq;  // no key, or none that counts
             const float inv = none ? 0.0f : 1.0f / l;
@@ -513,7 +523,7 @@ int prompt_attention(galois_b200_ctx* ctx, const void* q, const galois_dim* qd, 
         // a tensor without tokens is not read; a dimension of one element has any stride
         const uint64_t size[3] = {(uint64_t)qd->ne[0], (uint64_t)std::max<int64_t>(1, dims[i]->ne[2]), (uint64_t)dims[i]->ne[1]};
         const uint64_t stride[2] = {dims[i]->ne[2] > 1 ? (uint64_t)rows[i]->tok * 2 : 256, dims[i]->ne[1] > 1 ? (uint64_t)rows[i]->head * 2 : 256};
-        const uint32_t box[3] = {64, PT, 1};
+        const uint32_t box[3] = {64, (uint32_t)(i == 0 ? PT : KT), 1};
         const void* base = dims[i]->ne[2] > 0 ? (const void*)rows[i]->p : q;
         rc = gb_tensor_map(ctx, maps + i, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, base, size, stride, box, 128);
         if (rc) return rc;

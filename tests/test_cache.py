@@ -670,3 +670,133 @@ def test_a_slot_alone_gives_what_it_gives_in_a_batch(dev, G, hd, heads, kv):
         one = attend([p[s:s + 1] for p in parts], q[s:s + 1], lens[s:s + 1])
         _, bound, _, _ = R.step(q[s:s + 1], *[p[s:s + 1] for p in parts], lens[s:s + 1], 0.1)
         assert np.all(np.abs(one - whole[s:s + 1]) <= 2 * bound)
+
+
+# ------------------------------------------------------------------------------------------------ many, none, two at once
+
+
+@pytest.mark.parametrize("heads,kv", [(4, 2), (3, 1)])
+def test_prompt_attention_of_many_sequences(dev, G, heads, kv):
+    """More sequences than a warp has lanes, some without queries, some without keys."""
+    rng = np.random.default_rng(71)
+    seqs = [(int(a), int(max(0, a + b))) for a, b in zip(rng.integers(0, 40, 100), rng.integers(-20, 60, 100))]
+    seqs[40], seqs[77] = (700, 900), (130, 64)
+    q, k, v, qs, ks = prompt_inputs(rng, 64, heads, kv, seqs, 0)
+    out, bound = R.prompt(q, k, v, qs, ks, 0.125)
+    dst = put(G, np.full(q.shape, 3, np.float32))
+    gb.galois_prompt_attention(put(G, q), put(G, k), put(G, v), put(G, qs), put(G, ks), dst, 0.125)
+    dev.synchronize()
+    assert np.all(np.abs(dst.to_numpy() - out) <= bound)
+
+
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 1e-30])
+def test_prompt_attention_scales(dev, G, scale):
+    rng = np.random.default_rng(72)
+    q, k, v, qs, ks = prompt_inputs(rng, 128, 2, 1, [(150, 150), (3, 70)], 0)
+    out, _ = R.prompt(q, k, v, qs, ks, scale)
+    _, bound = R.prompt(q, k, v, qs, ks, abs(scale))
+    if scale < 0:  # the bound's probabilities belong to the other sign: all of them at once
+        bound = np.maximum(bound, 2.0**-10 * np.abs(v.astype(np.float64)).max())
+    dst = put(G, np.zeros(q.shape, np.float32))
+    gb.galois_prompt_attention(put(G, q), put(G, k), put(G, v), put(G, qs), put(G, ks), dst, scale)
+    dev.synchronize()
+    assert np.all(np.abs(dst.to_numpy() - out) <= bound)
+
+
+def test_nothing_to_see(dev, G):
+    """No keys at all, a cache without rows, no sequences, no tokens."""
+    q = put(G, np.ones((5, 2, 64), np.float16))
+    none = gb.Tensor.zeros((64, 2, 0), F16, G)
+    dst = put(G, np.full((5, 2, 64), 3, np.float32))
+    gb.galois_prompt_attention(q, none, none, put(G, np.array([0, 5], np.int32)), put(G, np.array([0, 0], np.int32)), dst, 0.1)
+    dev.synchronize()
+    assert not dst.to_numpy().any()
+    cache = gb.CacheQ8.zeros(64, 0, 2, 3, G)
+    q1, o1 = put(G, np.ones((3, 2, 64), np.float32)), put(G, np.full((3, 2, 64), 3, np.float32))
+    ws = gb.Tensor.zeros((gb.galois_cache_attention_workspace(cache, 2) // 4,), F32, G)
+    gb.galois_cache_attention(q1, cache, put(G, np.zeros(3, np.int32)), o1, 0.1, ws)
+    dev.synchronize()
+    assert not o1.to_numpy().any()
+    cache = gb.CacheQ8.zeros(64, 40, 2, 3, G)
+    kv = gb.Tensor.zeros((64, 2, 0), F32, G)
+    gb.galois_cache_append(kv, kv, put(G, np.zeros(4, np.int32)), put(G, np.zeros(3, np.int32)), cache)
+    cut = gb.CacheQ8.zeros(64, 0, 2, 3, G)
+    lens, ol = put(G, np.array([40, 1, 0], np.int32)), put(G, np.full(3, 9, np.int32))
+    empty_f, empty_i = gb.Tensor.zeros((0, 2, 3), F32, G), gb.Tensor.zeros((0, 2, 3), I32, G)
+    gb.galois_cache_evict(cache, lens, put(G, np.ones((3, 2, 40), np.float32)), 4, cut, ol, empty_f, empty_i)
+    dev.synchronize()
+    assert not ol.to_numpy().any()
+
+
+def test_cache_attention_of_many_slots(dev, G):
+    """More slots than a warp has lanes, most of them empty or short."""
+    rng = np.random.default_rng(73)
+    seqs, ctx = 150, 100
+    lens = rng.integers(0, 3, seqs) * rng.integers(0, 51, seqs)
+    lens[[0, 149]] = 0, 100
+    parts = random_cache(rng, seqs, 2, ctx, 64)
+    q, w = rng.normal(0, 1, (seqs, 18, 64)).astype(np.float32), rng.random((seqs, 2, ctx)).astype(np.float32)
+    out, bound, ww, wb = R.step(q, *parts, lens, 0.125, w)
+    cache, dst, wt = upload(G, parts), put(G, np.full_like(q, 3)), put(G, w)
+    ws = gb.Tensor.zeros((gb.galois_cache_attention_workspace(cache, 18, True) // 4,), F32, G)
+    gb.galois_cache_attention(put(G, q), cache, put(G, lens.astype(np.int32)), dst, 0.125, ws, weights=wt, weights_out=wt)
+    dev.synchronize()
+    assert np.all(np.abs(dst.to_numpy() - out) <= bound)
+    got = wt.to_numpy()
+    for s, n in enumerate(lens):
+        assert np.all(np.abs(got[s, :, :n] - ww[s, :, :n]) <= wb[s, :, :n]) and np.array_equal(got[s, :, n:], w[s, :, n:])
+
+
+def test_two_contexts_at_once(dev, G):
+    """Two contexts on streams of their own, their launches interleaved: each gives what it gives alone."""
+    import torch
+
+    rng = np.random.default_rng(74)
+    other = gb.CudaDevice(0, torch.cuda.Stream())
+    try:
+        places = [G, gb.Device.Gpu(other)]
+        lens = np.array([700, 300], np.int32)
+        work = []
+        for P in places:
+            parts = random_cache(rng, 2, 2, 700, 128)
+            q, k, v, qs, _ = prompt_inputs(rng, 128, 4, 2, [(260, 260), (90, 90)], 0)
+            q1 = rng.normal(0, 1, (2, 4, 128)).astype(np.float32)
+            t = {"cache": upload(P, parts), "q": put(P, q), "k": put(P, k), "v": put(P, v), "s": put(P, qs), "q1": put(P, q1), "l": put(P, lens),
+                 "o": put(P, np.zeros(q.shape, np.float16)), "o1": put(P, np.zeros_like(q1))}
+            t["ws"] = gb.Tensor.zeros((gb.galois_cache_attention_workspace(t["cache"], 4) // 4,), F32, P)
+            work.append((t, R.prompt(q, k, v, qs, qs, 0.09), R.step(q1, *parts, lens, 0.09)))
+        torch.cuda.synchronize()
+        for _ in range(20):
+            for t, _, _ in work:
+                gb.galois_prompt_attention(t["q"], t["k"], t["v"], t["s"], t["s"], t["o"], 0.09)
+                gb.galois_cache_attention(t["q1"], t["cache"], t["l"], t["o1"], 0.09, t["ws"])
+        dev.synchronize()
+        other.synchronize()
+        for t, (out, bound), (step, step_bound, _, _) in work:
+            assert np.all(np.abs(t["o"].to_numpy() - out) <= f16_bound(out, bound))
+            assert np.all(np.abs(t["o1"].to_numpy() - step) <= step_bound)
+    finally:
+        other.close()
+
+
+def test_beside_the_library_s_other_kernels(dev, G, oracle):
+    """Prompt attention between mat-muls that hold tensor memory themselves, all launched to overlap."""
+    rng = np.random.default_rng(75)
+    n = k = 256
+    w = oracle.quantize_q4_0(oracle.fill_normal(n * k, 170, 0, 0.02).reshape(n, k))
+    wt = gb.Tensor.from_raw(w, (k, n), GGmlType.Q4_0, G)
+    x = oracle.fill_normal(256 * k, 171).reshape(256, k)
+    xt, y1, y2 = put(G, x), gb.Tensor.zeros((n, 256), F32, G), gb.Tensor.zeros((n, 256), F32, G)
+    q, kk, v, qs, _ = prompt_inputs(rng, 64, 4, 4, [(256, 256)], 0)
+    qt, kt, vt, st, o = put(G, q), put(G, kk), put(G, v), put(G, qs), put(G, np.zeros(q.shape, np.float16))
+    for _ in range(5):
+        gb.galois_matmul(wt, xt, y1)
+        gb.galois_prompt_attention(qt, kt, vt, st, st, o, 0.125)
+        gb.galois_matmul(wt, xt, y2)
+    dev.synchronize()
+    assert np.array_equal(y1.to_numpy(), y2.to_numpy())
+    from conftest import assert_close
+
+    assert_close(y1.to_numpy(), oracle.mul_mat_q4_0(w, x))
+    out, bound = R.prompt(q, kk, v, qs, qs, 0.125)
+    assert np.all(np.abs(o.to_numpy() - out) <= f16_bound(out, bound))
