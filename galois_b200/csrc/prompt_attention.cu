@@ -9,7 +9,8 @@
 // exponentials (16 a cycle and SM against 32 pairs a cycle that the tensor cores get through).
 //
 //   warps 0-3, 4-7  soft-max of query tile 0, 1 (128 rows each, a thread per row)
-//   warp 8          loader: TMA copies of the query tiles, then keys and values, 64 rows at a time, through a ring of slots
+//   warp 8          loader: TMA copies of the query tiles, then keys and values, 64 rows at a time, through a ring; a slot of it
+//                   holds what one step takes, values j and keys j + 2 (the first: keys 0 and 1)
 //   warp 9          issues the tensor-core products and owns the tensor memory
 //   warp 10         clears what lies behind a sequence's end in its last tile of values
 //
@@ -75,8 +76,8 @@ template <int HD>
 struct plan {
     static constexpr uint32_t Q_TILE = PT * HD * 2, Q_HALF = PT * 128;  // bytes of a tile; of its first 64 columns
     static constexpr uint32_t TILE = KT * HD * 2, HALF = KT * 128;
-    static constexpr int SLOTS = HD == 128 ? 10 : 20;                   // tiles of keys and values in shared memory
-    static constexpr uint32_t Q = 0, KV = 2 * Q_TILE, BARS = KV + SLOTS * TILE, TOTAL = BARS + 512;
+    static constexpr int SLOTS = HD == 128 ? 5 : 10;                    // pairs of tiles of keys and values in shared memory
+    static constexpr uint32_t Q = 0, KV = 2 * Q_TILE, BARS = KV + SLOTS * 2 * TILE, TOTAL = BARS + 512;
     static_assert(TOTAL <= 227 * 1024, "shared memory");
 };
 struct prompt_args {
@@ -181,15 +182,14 @@ __global__ void __launch_bounds__(THREADS, 1)
     extern __shared__ __align__(1024) uint8_t smem[];  // swizzled tiles start at multiples of 1024
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
     uint64_t *q_full = bars, *q_free = bars + 1, *full = bars + 2, *empty = full + SLOTS, *s_full = empty + SLOTS, *p_ready = s_full + 4, *pv_done = p_ready + 4,
-             *v_raw = pv_done + 2;  // s_full, p_ready: [query tile][buffer]
+             *v_raw = pv_done + 4;  // [query tile][buffer]; pv_done: [query tile][last but one, last tile of a unit]
     uint32_t* tmem_at = reinterpret_cast<uint32_t*>(v_raw + 1);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) {
         tma_prefetch_map(&q_map), tma_prefetch_map(&k_map), tma_prefetch_map(&v_map);
         mbar_init(q_full, 1), mbar_init(q_free, 1), mbar_init(v_raw, 1);
         for (int i = 0; i < SLOTS; i++) mbar_init(full + i, 1), mbar_init(empty + i, 1);
-        for (int i = 0; i < 4; i++) mbar_init(s_full + i, 1), mbar_init(p_ready + i, 4);
-        for (int i = 0; i < 2; i++) mbar_init(pv_done + i, 1);
+        for (int i = 0; i < 4; i++) mbar_init(s_full + i, 1), mbar_init(p_ready + i, 4), mbar_init(pv_done + i, 1);
         fence_mbarrier_init_cluster();
     }
     if (warp == ISSUER) {
@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     bool fine = true;
 
     if (warp == LOADER) {
-        int it = 0, nu = 0;  // tiles of keys and values so far, units with any
+        int it = 0, nu = 0;  // slots filled so far, units with any keys
         for (int r = 0; fine && x.find(p, f, unit_of_round(r), units, span, two_heads); r++) {
             if (x.n == 0) continue;
             if (lane == 0) {
@@ -222,18 +222,19 @@ __global__ void __launch_bounds__(THREADS, 1)
                             tma_load_3d(smem_u32(smem + L::Q) + s * L::Q_TILE + h * L::Q_HALF, &q_map, 64 * h, x.q0 + x.first + (two_heads ? 0 : s * PT),
                                         two_heads ? x.head0 + s : x.head0, q_full);
                 }
-                // in the order of their use: two tiles of keys, then values and the keys after next in turn
-                for (int i = 0; i < 2 * x.n && fine; i++, it++) {
-                    const bool keys = i == 0 || (i == 1 && x.n > 1) || ((i & 1) && (i >> 1) + 1 < x.n);
-                    const int tile = i < 2 ? (keys ? i : 0) : (i & 1) ? (keys ? (i >> 1) + 1 : i >> 1) : (i >> 1) - 1;
+                for (int i = 0; i <= x.n && fine; i++, it++) {
                     const int slot = it % SLOTS;
                     if (it >= SLOTS) fine = mbar_try_bounded(empty + slot, (it / SLOTS - 1) & 1);
                     if (!fine) break;
                     // a last tile of values that warp 10 has to clear arrives at a barrier of its own; it passes the tile on
-                    uint64_t* bar = i == 2 * x.n - 1 && x.ragged() ? v_raw : full + slot;
-                    mbar_expect_tx(bar, L::TILE);
-                    for (int h = 0; h < HD / 64; h++)
-                        tma_load_3d(smem_u32(smem + L::KV) + slot * L::TILE + h * L::HALF, keys ? &k_map : &v_map, 64 * h, x.k0 + tile * KT, x.kh, bar);
+                    uint64_t* bar = i == x.n && x.ragged() ? v_raw : full + slot;
+                    const bool second = i + 1 < x.n;  // keys i + 1 exist
+                    mbar_expect_tx(bar, second ? 2 * L::TILE : L::TILE);
+                    const uint32_t to = smem_u32(smem + L::KV) + slot * 2 * L::TILE;
+                    for (int h = 0; h < HD / 64; h++) {
+                        tma_load_3d(to + h * L::HALF, i == 0 ? &k_map : &v_map, 64 * h, x.k0 + (i == 0 ? 0 : i - 1) * KT, x.kh, bar);
+                        if (second) tma_load_3d(to + L::TILE + h * L::HALF, &k_map, 64 * h, x.k0 + (i + 1) * KT, x.kh, bar);
+                    }
                 }
             }
             nu++;
@@ -262,8 +263,8 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (++slot == SLOTS) slot = 0, parity ^= 1;
         };
         auto wait = [&](uint64_t* bar, uint32_t phase) { return __all_sync(0xffffffffu, mbar_try_bounded(bar, phase)) != 0; };
-        auto logits = [&](int s, int b) {  // of the keys in `slot`, into buffer b
-            const uint64_t q = q_desc + (uint32_t)(s * (L::Q_TILE >> 4)), k = k_desc + (uint32_t)(slot * (L::TILE >> 4));
+        auto logits = [&](int s, int b, uint64_t k) {  // of the keys at k, into buffer b
+            const uint64_t q = q_desc + (uint32_t)(s * (L::Q_TILE >> 4));
 #pragma unroll
             for (int kk = 0; kk < HD / 16; kk++) {
                 constexpr uint32_t QH = L::Q_HALF >> 4, KH = L::HALF >> 4;
@@ -273,49 +274,42 @@ __global__ void __launch_bounds__(THREADS, 1)
         };
         for (int r = 0; fine && x.find(p, f, unit_of_round(r), units, span, two_heads); r++) {
             if (x.n == 0) continue;
-            fine = wait(q_full, q_parity);
+            fine = wait(q_full, q_parity) && wait(full + slot, parity);
             q_parity ^= 1;
-            for (int b = 0; b < 2 && b < x.n && fine; b++) {
+            if (!fine) break;
+            // Both buffers of one query tile, then of the other: the second soft-max starts half a step behind the first, and
+            // the special-function unit is asked for by one at a time.
+            const uint64_t k0 = k_desc + (uint32_t)(2 * slot * (L::TILE >> 4)), k1 = k0 + (L::TILE >> 4);
+            if (x.tiles0 > 0) logits(0, 0, k0);
+            if (x.tiles0 > 1) logits(0, 1, k1);
+            if (x.tiles1 > 0) logits(1, 0, k0);
+            if (x.tiles1 > 1) logits(1, 1, k1);
+            tc_commit(empty + slot, lead);
+            next();
+            if (x.n <= 2) tc_commit(q_free, lead);  // the queries have been used for the last time
+            for (int j = 0; j < x.n; j++) {
+                const int b = j & 1;
+                const uint64_t v = v_desc + (uint32_t)(2 * slot * (L::TILE >> 4)), k = k_desc + (uint32_t)((2 * slot + 1) * (L::TILE >> 4));
                 fine = wait(full + slot, parity);
-                if (!fine) break;
-                if (x.tiles0 > b) logits(0, b);
-                if (x.tiles1 > b) logits(1, b);
-                tc_commit(empty + slot, lead);
-                next();
-            }
-            if (fine && x.n <= 2) tc_commit(q_free, lead);  // the queries have been used for the last time
-            for (int j = 0; j < x.n && fine; j++) {
-                const int vs = slot, b = j & 1;
-                fine = wait(full + vs, parity);
-                next();
-                const bool more = j + 2 < x.n;  // the keys after next lie in `slot`
-                bool keys = false;              // they have arrived
 #pragma unroll
                 for (int s = 0; s < 2; s++) {
                     const int tiles = s ? x.tiles1 : x.tiles0;
                     if (j >= tiles || !fine) continue;
                     fine = wait(p_ready + 2 * s + b, (ready >> (2 * s + b)) & 1);
                     ready ^= 1u << (2 * s + b);
-                    if (!fine) break;
+                    if (!fine) continue;
                     tc_after_sync();
-                    const uint64_t v = v_desc + (uint32_t)(vs * (L::TILE >> 4));
 #pragma unroll
                     for (int kk = 0; kk < KT / 16; kk++)
                         tc_mma_f16_ts(tmem + 2 * PT + s * HD, tmem + s * PT + b * KT + kk * 8, v + kk * (2048 >> 4), idesc_o, j > 0 || kk > 0, lead);
-                    tc_commit(pv_done + s, lead);
-                    if (s == 1 || j >= x.tiles1) tc_commit(empty + vs, lead);
-                    if (j + 2 < tiles) {
-                        if (!keys) fine = wait(full + slot, parity);
-                        if (!fine) break;
-                        keys = true;
-                        logits(s, b);
-                    }
+                    // logits j + 2 come after these products, so their barrier speaks for both
+                    if (j + 2 < tiles) logits(s, b, k);
+                    else tc_commit(pv_done + 2 * s + (j + 1 == tiles), lead);
                 }
-                if (fine && more) {
-                    tc_commit(empty + slot, lead);
-                    next();
-                    if (j + 3 == x.n) tc_commit(q_free, lead);
-                }
+                if (!fine) break;
+                tc_commit(empty + slot, lead);
+                next();
+                if (j + 3 == x.n) tc_commit(q_free, lead);
             }
         }
     } else if (warp == CLEARER) {
@@ -326,13 +320,13 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         int it = 0, nr = 0;
         for (int r = 0; fine && x.find(p, f, unit_of_round(r), units, span, two_heads); r++) {
-            it += 2 * x.n;
+            it += x.n > 0 ? x.n + 1 : 0;
             if (!x.ragged()) continue;
             fine = __all_sync(0xffffffffu, mbar_try_bounded(v_raw, nr & 1));
             nr++;
             if (!fine) break;
             const int slot = (it - 1) % SLOTS, valid = x.nk - (x.n - 1) * KT;
-            uint4* v = reinterpret_cast<uint4*>(smem + L::KV + slot * L::TILE);  // [half][row][8 pieces]
+            uint4* v = reinterpret_cast<uint4*>(smem + L::KV + slot * 2 * L::TILE);  // [half][row][8 pieces]
             for (int h = 0; h < HD / 64; h++)
                 for (int i = valid * 8 + lane; i < KT * 8; i += 32) v[h * KT * 8 + i] = make_uint4(0, 0, 0, 0);
             fence_proxy_async();
@@ -346,7 +340,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const uint32_t s_at = tmem + s * PT + lanes, o_at = tmem + 2 * PT + s * HD + lanes;
         const float c = fmaxf(fabsf(p.scale) * 1.4426950408889634f, 1e-30f);  // not 0: a masked logit stays below all others
         const bool flip = p.scale < 0.0f;
-        uint32_t nt = 0, done = 0;  // bit b: parity of the next logits in buffer b; key tiles of all units so far
+        uint32_t nt = 0, done = 0;  // bit b: parity of the next logits in buffer b; the next last but one, the next last products
         for (int r = 0;; r++) {
             const int64_t u = unit_of_round(r);
             // The unit is looked up here and again for the results: what describes it does not stay in registers.
@@ -402,7 +396,9 @@ __global__ void __launch_bounds__(THREADS, 1)
                     if (raise) top = most;
                     l *= keep;
                     if (j > 0) {
-                        fine = fine && __all_sync(0xffffffffu, mbar_try_bounded(pv_done + s, (done + j - 1) & 1));
+                        // products j - 1 are done: logits j + 1 come after them, or else a barrier of their own says so
+                        const bool ok = j + 1 < mine ? mbar_try_bounded(s_full + 2 * s + (b ^ 1), (nt >> (b ^ 1)) & 1) : mbar_try_bounded(pv_done + 2 * s, done & 1);
+                        fine = fine && __all_sync(0xffffffffu, ok);
                         tc_after_sync();
 #pragma unroll
                         for (int i = 0; i < HD / 32; i++) {
@@ -424,12 +420,12 @@ __global__ void __launch_bounds__(THREADS, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_ready + 2 * s + b);
             }
-            done += mine;
             // ---- results
             f.start(p, span);
             x.find(p, f, u, units, span, two_heads);
             const int at = x.first + (two_heads ? 0 : s * PT) + row;
-            if (mine > 0) fine = fine && __all_sync(0xffffffffu, mbar_try_bounded(pv_done + s, (done - 1) & 1));
+            if (mine > 0) fine = fine && __all_sync(0xffffffffu, mbar_try_bounded(pv_done + 2 * s + 1, done >> 1));
+            done ^= mine > 1 ? 3u : mine > 0 ? 2u : 0u;
             tc_after_sync();
             const bool none = top == -INFINITY, live = fine && at < x.nq;  // no key, or none that counts
             const float inv = none ? 0.0f : 1.0f / l;
