@@ -188,12 +188,12 @@ __global__ void __launch_bounds__(THREADS, 1)
     extern __shared__ __align__(1024) uint8_t smem[];  // swizzled tiles start at multiples of 1024
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
     uint64_t *q_full = bars, *q_free = bars + 1, *full = bars + 2, *empty = full + SLOTS, *s_full = empty + SLOTS, *p_ready = s_full + 4, *pv_done = p_ready + 4,
-             *v_raw = pv_done + 4;  // [query tile][buffer]; pv_done: [query tile][last but one, last tile of a unit]
-    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(v_raw + 1);
+             *v_raw = pv_done + 4;  // [query tile][buffer]; pv_done: [query tile][last but one, last tile of a unit]; v_raw: the units that are ragged in turn
+    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(v_raw + 2);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) {
         tma_prefetch_map(&q_map), tma_prefetch_map(&k_map), tma_prefetch_map(&v_map);
-        mbar_init(q_full, 1), mbar_init(q_free, 1), mbar_init(v_raw, 1);
+        mbar_init(q_full, 1), mbar_init(q_free, 1), mbar_init(v_raw, 1), mbar_init(v_raw + 1, 1);
         for (int i = 0; i < SLOTS; i++) mbar_init(full + i, 1), mbar_init(empty + i, 1);
         for (int i = 0; i < 4; i++) mbar_init(s_full + i, 1), mbar_init(p_ready + i, 4), mbar_init(pv_done + i, 1);
         fence_mbarrier_init_cluster();
@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     bool fine = true;
 
     if (warp == LOADER) {
-        int it = 0, nu = 0;  // slots filled so far, units with any keys
+        int it = 0, nu = 0, nr = 0;  // slots filled so far, units with any keys, ragged ones
         for (int r = 0; fine && x.find(p, f, unit_of_round(r), units, span, two_heads); r++) {
             if (x.n == 0) continue;
             if (lane == 0) {
@@ -232,8 +232,10 @@ __global__ void __launch_bounds__(THREADS, 1)
                     const int slot = it % SLOTS;
                     if (it >= SLOTS) fine = mbar_try_bounded(empty + slot, (it / SLOTS - 1) & 1);
                     if (!fine) break;
-                    // a last tile of values that warp 10 has to clear arrives at a barrier of its own; it passes the tile on
-                    uint64_t* bar = i == x.n && x.ragged() ? v_raw : full + slot;
+                    // A last tile of values that warp 10 has to clear arrives at a barrier of its own, and warp 10 passes the tile on.
+                    // Two such tiles can be under way: this unit's and the one's before, whose values are not waited for here.
+                    // The one's before that has been passed on, as its products came before the logits that q_free speaks for.
+                    uint64_t* bar = i == x.n && x.ragged() ? v_raw + (nr & 1) : full + slot;
                     const bool second = i + 1 < x.n;  // keys i + 1 exist
                     mbar_expect_tx(bar, second ? 2 * L::TILE : L::TILE);
                     const uint32_t to = smem_u32(smem + L::KV) + slot * 2 * L::TILE;
@@ -244,6 +246,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
             }
             nu++;
+            nr += x.ragged();
             fine = __shfl_sync(0xffffffffu, (int)fine, 0);
         }
         // no arrival and no copy is left under way: the last tiles have been used (or, after a time-out, have had time to land)
@@ -283,8 +286,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             fine = wait(q_full, q_parity) && wait(full + slot, parity);
             q_parity ^= 1;
             if (!fine) break;
-            // Both buffers of one query tile, then of the other: the second soft-max starts half a step behind the first, and
-            // the special-function unit is asked for by one at a time.
+            // both buffers of one query tile, then of the other (the other order takes as long)
             const uint64_t k0 = k_desc + (uint32_t)(2 * slot * (L::TILE >> 4)), k1 = k0 + (L::TILE >> 4);
             if (x.tiles0 > 0) logits(0, 0, k0);
             if (x.tiles0 > 1) logits(0, 1, k1);
@@ -328,7 +330,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int r = 0; fine && x.find(p, f, unit_of_round(r), units, span, two_heads); r++) {
             it += x.n > 0 ? x.n + 1 : 0;
             if (!x.ragged()) continue;
-            fine = __all_sync(0xffffffffu, mbar_try_bounded(v_raw, nr & 1));
+            fine = __all_sync(0xffffffffu, mbar_try_bounded(v_raw + (nr & 1), (nr >> 1) & 1));
             nr++;
             if (!fine) break;
             const int slot = (it - 1) % SLOTS, valid = x.nk - (x.n - 1) * KT;

@@ -800,3 +800,20 @@ def test_beside_the_library_s_other_kernels(dev, G, oracle):
     assert_close(y1.to_numpy(), oracle.mul_mat_q4_0(w, x))
     out, bound = R.prompt(q, kk, v, qs, qs, 0.125)
     assert np.all(np.abs(o.to_numpy() - out) <= f16_bound(out, bound))
+
+
+@pytest.mark.parametrize("hd,heads,kv", [(64, 4, 2), (128, 2, 2)])
+def test_prompt_attention_of_short_ragged_prompts_one_after_the_other(dev, G, hd, heads, kv):
+    """Every unit is one ragged tile of keys, and each SM goes through several of them: the next unit's values may be under way
+    before this one's have arrived.  Each replay finds its operands in HBM."""
+    rng = np.random.default_rng(74)
+    seqs = [(int(n), int(n)) for n in rng.integers(1, 61, 700)]
+    q, k, v, qs, ks = prompt_inputs(rng, hd, heads, kv, seqs, 0)
+    args = [put(G, a) for a in (q, k, v, qs, ks)]
+    dst = put(G, np.full(q.shape, 3, np.float32))
+    out, bound = R.prompt(q, k, v, qs, ks, 0.125)
+    for _ in range(3):
+        gb.Tensor.zeros((1 << 26,), F32, G)  # 256 MB pass through L2
+        gb.galois_prompt_attention(*args, dst, 0.125)
+        dev.synchronize()
+        assert np.all(np.abs(dst.to_numpy() - out) <= bound)
