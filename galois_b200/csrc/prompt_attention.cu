@@ -115,6 +115,21 @@ __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
 __device__ __forceinline__ float f2_low(uint64_t a) { return __uint_as_float((uint32_t)a); }
 __device__ __forceinline__ float f2_high(uint64_t a) { return __uint_as_float((uint32_t)(a >> 32)); }
 
+// Bounded wait.  How long another role may rightly take is the length of the prompt's matter (a unit of a million keys, rows
+// formed by the plain loop), so the limit is on time in which nobody reports progress: the issuer now and then, the plain
+// loop after each row.
+__device__ __forceinline__ bool arrived(uint64_t* bar, uint32_t parity, const volatile uint32_t* progress) {
+    if (mbar_try(bar, parity)) return true;
+    uint32_t seen = *progress;
+    long long t0 = clock64();
+    while (!mbar_try(bar, parity)) {
+        if (clock64() - t0 <= (1ll << 32)) continue;
+        if (*progress == seen) return false;
+        seen = *progress, t0 = clock64();
+    }
+    return true;
+}
+
 // What of a sequence's starts can be used: queries [q0, q0 + nq), keys [k0, k0 + nk); false if they are out of range.
 __device__ __forceinline__ bool sequence(const prompt_args& p, int s, int& q0, int& nq, int& k0, int& nk) {
     q0 = p.q_starts[s], k0 = p.k_starts[s];
@@ -189,9 +204,10 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
     uint64_t *q_full = bars, *q_free = bars + 1, *full = bars + 2, *empty = full + SLOTS, *s_full = empty + SLOTS, *p_ready = s_full + 4, *pv_done = p_ready + 4,
              *v_raw = pv_done + 4;  // [query tile][buffer]; pv_done: [query tile][last but one, last tile of a unit]; v_raw: the units that are ragged in turn
-    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(v_raw + 2);
+    uint32_t *tmem_at = reinterpret_cast<uint32_t*>(v_raw + 2), *progress = tmem_at + 1;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) {
+        *progress = 0;
         tma_prefetch_map(&q_map), tma_prefetch_map(&k_map), tma_prefetch_map(&v_map);
         mbar_init(q_full, 1), mbar_init(q_free, 1), mbar_init(v_raw, 1), mbar_init(v_raw + 1, 1);
         for (int i = 0; i < SLOTS; i++) mbar_init(full + i, 1), mbar_init(empty + i, 1);
@@ -220,7 +236,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int r = 0; fine && x.find(p, f, unit_of_round(r), units, span, two_heads); r++) {
             if (x.n == 0) continue;
             if (lane == 0) {
-                if (nu > 0) fine = mbar_try_bounded(q_free, (nu - 1) & 1);
+                if (nu > 0) fine = arrived(q_free, (nu - 1) & 1, progress);
                 if (fine) {
                     mbar_expect_tx(q_full, 2 * L::Q_TILE);
                     for (int s = 0; s < 2; s++)
@@ -230,7 +246,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
                 for (int i = 0; i <= x.n && fine; i++, it++) {
                     const int slot = it % SLOTS;
-                    if (it >= SLOTS) fine = mbar_try_bounded(empty + slot, (it / SLOTS - 1) & 1);
+                    if (it >= SLOTS) fine = arrived(empty + slot, (it / SLOTS - 1) & 1, progress);
                     if (!fine) break;
                     // A last tile of values that warp 10 has to clear arrives at a barrier of its own, and warp 10 passes the tile on.
                     // Two such tiles can be under way: this unit's and the one's before, whose values are not waited for here.
@@ -252,10 +268,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         // no arrival and no copy is left under way: the last tiles have been used (or, after a time-out, have had time to land)
         if (lane == 0) {
             for (int i = max(0, it - SLOTS); i < it; i++) {
-                if (fine) fine = mbar_try_bounded(empty + i % SLOTS, (i / SLOTS) & 1);
-                else mbar_try_bounded(full + i % SLOTS, (i / SLOTS) & 1);
+                if (fine) fine = arrived(empty + i % SLOTS, (i / SLOTS) & 1, progress);
+                else arrived(full + i % SLOTS, (i / SLOTS) & 1, progress);
             }
-            if (fine && nu > 0) fine = mbar_try_bounded(q_free, (nu - 1) & 1);
+            if (fine && nu > 0) fine = arrived(q_free, (nu - 1) & 1, progress);
         }
     } else if (warp == ISSUER) {
         // f32 sums, F16 operands; logits: keys as they are; results: values with the contraction along their rows
@@ -271,7 +287,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         auto next = [&]() {
             if (++slot == SLOTS) slot = 0, parity ^= 1;
         };
-        auto wait = [&](uint64_t* bar, uint32_t phase) { return __all_sync(0xffffffffu, mbar_try_bounded(bar, phase)) != 0; };
+        auto wait = [&](uint64_t* bar, uint32_t phase) { return __all_sync(0xffffffffu, arrived(bar, phase, progress)) != 0; };
         auto logits = [&](int s, int b, uint64_t k) {  // of the keys at k, into buffer b
             const uint64_t q = q_desc + (uint32_t)(s * (L::Q_TILE >> 4));
 #pragma unroll
@@ -299,6 +315,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 const int b = j & 1;
                 const uint64_t v = v_desc + (uint32_t)(2 * slot * (L::TILE >> 4)), k = k_desc + (uint32_t)((2 * slot + 1) * (L::TILE >> 4));
                 fine = wait(full + slot, parity);
+                if ((j & 1023) == 0 && lead) atomicAdd(progress, 1u);
 #pragma unroll
                 for (int s = 0; s < 2; s++) {
                     const int tiles = s ? x.tiles1 : x.tiles0;
@@ -330,7 +347,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int r = 0; fine && x.find(p, f, unit_of_round(r), units, span, two_heads); r++) {
             it += x.n > 0 ? x.n + 1 : 0;
             if (!x.ragged()) continue;
-            fine = __all_sync(0xffffffffu, mbar_try_bounded(v_raw + (nr & 1), (nr >> 1) & 1));
+            fine = __all_sync(0xffffffffu, arrived(v_raw + (nr & 1), (nr >> 1) & 1, progress));
             nr++;
             if (!fine) break;
             const int slot = (it - 1) % SLOTS, valid = x.nk - (x.n - 1) * KT;
@@ -360,7 +377,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             float top = -INFINITY, l = 0.0f;  // what the probabilities refer to, their sum
             for (int j = 0; j < mine; j++) {
                 const uint32_t b = j & 1, b_at = s_at + b * KT;
-                fine = fine && __all_sync(0xffffffffu, mbar_try_bounded(s_full + 2 * s + b, (nt >> b) & 1));
+                fine = fine && __all_sync(0xffffffffu, arrived(s_full + 2 * s + b, (nt >> b) & 1, progress));
                 nt ^= 1u << b;
                 tc_after_sync();
                 float y[KT];
@@ -405,7 +422,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     l *= keep;
                     if (j > 0) {
                         // products j - 1 are done: logits j + 1 come after them, or else a barrier of their own says so
-                        const bool ok = j + 1 < mine ? mbar_try_bounded(s_full + 2 * s + (b ^ 1), (nt >> (b ^ 1)) & 1) : mbar_try_bounded(pv_done + 2 * s, done & 1);
+                        const bool ok = j + 1 < mine ? arrived(s_full + 2 * s + (b ^ 1), (nt >> (b ^ 1)) & 1, progress) : arrived(pv_done + 2 * s, done & 1, progress);
                         fine = fine && __all_sync(0xffffffffu, ok);
                         tc_after_sync();
 #pragma unroll
@@ -432,7 +449,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             f.start(p, span);
             x.find(p, f, u, units, span, two_heads);
             const int at = x.first + (two_heads ? 0 : s * PT) + row;
-            if (mine > 0) fine = fine && __all_sync(0xffffffffu, mbar_try_bounded(pv_done + 2 * s + 1, done >> 1));
+            if (mine > 0) fine = fine && __all_sync(0xffffffffu, arrived(pv_done + 2 * s + 1, done >> 1, progress));
             done ^= mine > 1 ? 3u : mine > 0 ? 2u : 0u;
             tc_after_sync();
             const bool none = top == -INFINITY, live = fine && at < x.nq;  // no key, or none that counts
@@ -464,12 +481,11 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
             }
             tc_before_sync();
-            // this warp's rows by the plain loop, where a result is not finite
-            if (__any_sync(0xffffffffu, live && (odd >> 31))) {
-                for (int w = 0; w < 32; w++) {
-                    const int i = at - lane + w, key = i + x.nk - x.nq + 1;
-                    if (i < x.nq) prompt_row<HD, T>(p.q, p.k, p.v, x.q0 + i, x.k0, key, head, x.kh, p.scale, out + (int64_t)(row - lane + w) * p.o_tok);
-                }
+            // rows whose result is not finite, by the plain loop
+            for (uint32_t rows = __ballot_sync(0xffffffffu, live && (odd >> 31)); rows; rows &= rows - 1) {
+                const int w = __ffs(rows) - 1, i = at - lane + w, key = i + x.nk - x.nq + 1;
+                prompt_row<HD, T>(p.q, p.k, p.v, x.q0 + i, x.k0, key, head, x.kh, p.scale, out + (int64_t)(row - lane + w) * p.o_tok);
+                if (lane == 0) atomicAdd(progress, 1u);
             }
         }
     }

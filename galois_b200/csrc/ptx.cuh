@@ -71,15 +71,6 @@ __device__ __forceinline__ bool mbar_try(uint64_t* bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-// The bounded wait made of those.
-__device__ __forceinline__ bool mbar_try_bounded(uint64_t* bar, uint32_t parity) {
-    if (mbar_try(bar, parity)) return true;
-    const long long t0 = clock64();
-    while (!mbar_try(bar, parity)) {
-        if (clock64() - t0 > (1ll << 32)) return false;
-    }
-    return true;
-}
 // 1-D bulk copy global -> this CTA's shared memory, completing on an mbarrier.  Both addresses
 // 16-byte aligned, size a multiple of 16 bytes.  No multicast.
 __device__ __forceinline__ void bulk_g2s(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
