@@ -71,6 +71,10 @@ __global__ void __launch_bounds__(128) cache_append_kernel(const T* __restrict__
         const int s = gb_find_seq(starts, nseq, t);
         if (s >= nseq) break;  // behind the last sequence
         const int begin = starts[s], end = starts[s + 1], p0 = pos[s];
+        if (s == 0 && begin > t && end >= begin && end <= tokens) {  // in front of the first sequence
+            t = begin;
+            continue;
+        }
         if (begin < 0 || begin > t || end <= t || end > tokens || p0 < 0 || p0 > c.ctx - (end - begin)) {
             if (threadIdx.x == 0) *status = GALOIS_B200_E_BADARG;  // nothing of this sequence is written
             t = end > t ? end : t + 1;
@@ -167,7 +171,7 @@ __global__ void __launch_bounds__(128) cache_read_kernel(gb_cache_view c, const 
     uint32_t w[N][W];
     float d[N];
     bool live[N];
-    if (s < nseq && begin >= 0 && begin <= tile && end >= tile + READ_ROWS && end <= tokens && p0 >= 0 && p0 <= c.ctx - READ_ROWS - (tile - begin)) {
+    if (s < nseq && begin >= 0 && begin <= tile && end >= tile + READ_ROWS && end <= tokens && p0 >= 0 && p0 <= c.ctx - (end - begin)) {
         // all rows of one sequence
         const int p = p0 + (t0 - begin);
         const int8_t* from = q + s * c.seq + p * c.tok;
@@ -191,8 +195,9 @@ __global__ void __launch_bounds__(128) cache_read_kernel(gb_cache_view c, const 
             while (s < nseq && end <= t) {
                 if (++s < nseq) begin = end, end = starts[s + 1], p0 = pos[s];
             }
-            if (t < tokens && s < nseq) {
-                if (begin < 0 || begin > t || end > tokens || p0 < 0 || p0 >= c.ctx - (t - begin)) {
+            const bool front = s == 0 && begin > t && end >= begin && end <= tokens;  // of the first sequence
+            if (t < tokens && s < nseq && !front) {
+                if (begin < 0 || begin > t || end > tokens || p0 < 0 || p0 > c.ctx - (end - begin)) {
                     *status = GALOIS_B200_E_BADARG;
                 } else {
                     const int p = p0 + (t - begin);
@@ -444,8 +449,9 @@ int append(galois_b200_ctx* ctx, const char* what, const galois_b200_cache_q8* c
     if (rc == 0) rc = check_packed(ctx, what, starts, pos, nseq, c);
     if (rc) return rc;
     if (kd->ne[2] != vd->ne[2]) return gb_fail(ctx, GALOIS_B200_E_SHAPE, "%s: k and v hold different numbers of tokens", what);
-    if (touches(c, cache, k, gb_span(kd, sizeof(T))) || touches(c, cache, v, gb_span(vd, sizeof(T))))
-        return gb_fail(ctx, GALOIS_B200_E_BADARG, "%s: the new rows lie in the cache", what);
+    if (touches(c, cache, k, gb_span(kd, sizeof(T))) || touches(c, cache, v, gb_span(vd, sizeof(T))) || touches(c, cache, starts, 4 * ((size_t)nseq + 1)) ||
+        touches(c, cache, pos, 4 * (size_t)nseq))
+        return gb_fail(ctx, GALOIS_B200_E_BADARG, "%s: the operands lie in the cache", what);
     const int tokens = (int)kd->ne[2];
     if (tokens == 0 || nseq == 0 || c.kv_heads == 0) return 0;
     gb_on_device on(ctx);
@@ -469,8 +475,10 @@ int read_rows(galois_b200_ctx* ctx, const char* what, const galois_b200_cache_q8
     if (rc) return rc;
     if (kd->ne[2] != vd->ne[2]) return gb_fail(ctx, GALOIS_B200_E_SHAPE, "%s: k and v hold different numbers of tokens", what);
     const size_t kn = gb_span(kd, sizeof(T)), vn = gb_span(vd, sizeof(T));
-    if (touches(c, cache, k, kn) || touches(c, cache, v, vn) || gb_overlap(k, kn, v, vn))
-        return gb_fail(ctx, GALOIS_B200_E_DST, "%s: the destinations overlap each other or the cache", what);
+    const size_t sn = 4 * ((size_t)nseq + 1), pn = 4 * (size_t)nseq;
+    if (touches(c, cache, k, kn) || touches(c, cache, v, vn) || gb_overlap(k, kn, v, vn) || gb_overlap(k, kn, starts, sn) || gb_overlap(k, kn, pos, pn) ||
+        gb_overlap(v, vn, starts, sn) || gb_overlap(v, vn, pos, pn))
+        return gb_fail(ctx, GALOIS_B200_E_DST, "%s: the destinations overlap each other or the operands", what);
     const int tokens = (int)kd->ne[2];
     if (tokens == 0 || nseq == 0 || c.kv_heads == 0) return 0;
     gb_on_device on(ctx);

@@ -817,3 +817,52 @@ def test_prompt_attention_of_short_ragged_prompts_one_after_the_other(dev, G, hd
         gb.galois_prompt_attention(*args, dst, 0.125)
         dev.synchronize()
         assert np.all(np.abs(dst.to_numpy() - out) <= bound)
+
+
+@pytest.mark.parametrize("first,lens,pos", [(3, [5, 40], [30, 0]), (64, [1, 1], [0, 63]), (45, [64], [0])])
+def test_rows_in_front_of_the_first_sequence(dev, G, first, lens, pos):
+    """starts need not begin at 0: what lies in front belongs to nobody, and is no error."""
+    rng = np.random.default_rng(75)
+    starts = R.starts_of(lens) + first
+    tokens = int(starts[-1]) + 2
+    parts = random_cache(rng, len(lens), 2, 64, 64)
+    x = [rng.normal(0, 1, (tokens, 2, 64)).astype(np.float32) for _ in range(2)]
+    cache, want = upload(G, parts), [p.copy() for p in parts]
+    s, p = put(G, starts.astype(np.int32)), put(G, np.array(pos, np.int32))
+    gb.galois_cache_append(put(G, x[0]), put(G, x[1]), s, p, cache)
+    outs = [put(G, np.full((tokens, 2, 64), 9, np.float32)) for _ in range(2)]
+    gb.galois_cache_read(cache, s, p, outs[0], outs[1])
+    dev.synchronize()
+    for h in range(2):
+        R.append(x[h][first:], starts - first, pos, want[2 * h], want[2 * h + 1])
+    for got, w in zip(parts_of(cache, want), want):
+        assert np.array_equal(got, w)
+    for h, out in enumerate(outs):
+        rows, got = R.values(want[2 * h], want[2 * h + 1]), out.to_numpy()
+        assert np.all(got[:first] == 9) and np.all(got[starts[-1]:] == 9)
+        for i, n in enumerate(lens):
+            assert np.array_equal(got[starts[i]:starts[i + 1]], rows[i, :, pos[i]:pos[i] + n].transpose(1, 0, 2).astype(np.float32))
+
+
+@pytest.mark.parametrize("starts", [[4, 2, 5], [5, 7, 7], [9, 9, 9]])
+def test_starts_that_do_not_ascend_or_pass_the_end_are_reported(dev, G, starts):
+    cache = upload(G, random_cache(np.random.default_rng(76), 2, 1, 64, 64))
+    x = put(G, np.ones((5, 1, 64), np.float32))
+    s, p = put(G, np.array(starts, np.int32)), put(G, np.zeros(2, np.int32))
+    gb.galois_cache_append(x, x, s, p, cache)
+    with pytest.raises(GError) as e:
+        dev.synchronize()
+    assert e.value.code == -1
+
+
+@pytest.mark.parametrize("n", [3, 70])
+def test_read_leaves_a_sequence_out_as_a_whole(dev, G, n):
+    """One row too many for the slot: none of the sequence's rows is written."""
+    cache = upload(G, random_cache(np.random.default_rng(77), 2, 1, 100, 64))
+    outs = [put(G, np.full((n + 2, 1, 64), 9, np.float32)) for _ in range(2)]
+    gb.galois_cache_read(cache, put(G, np.array([0, n, n + 2], np.int32)), put(G, np.array([101 - n, 5], np.int32)), outs[0], outs[1])
+    with pytest.raises(GError):
+        dev.synchronize()
+    for out in outs:
+        got = out.to_numpy()
+        assert np.all(got[:n] == 9) and not np.any(got[n:] == 9)

@@ -171,3 +171,11 @@ def test_cpu_tensors_are_refused():
     with pytest.raises(GError):
         gb.galois_prompt_attention(h, h, h, i, i, h, 1.0)
     assert np.array_equal(z(4, t=GGmlType.I8).to_numpy(), np.zeros(4, np.int8))
+
+
+def test_metadata_inside_what_is_written_is_refused(ctx):
+    assert append(ctx, cache(), starts=C.c_void_p((1 << 40) + 64)) == BADARG
+    assert append(ctx, cache(), pos=C.c_void_p((4 << 40) + 4)) == BADARG
+    kd = rows()
+    for a, b in ((1, 4), (3, 1), (2, 4), (3, 2)):  # starts, positions: in k, in k, in v, in v
+        assert lib.galois_b200_cache_read_f32(ctx, C.byref(cache()), addr(a), addr(b), 3, addr(1), C.byref(kd), addr(2), C.byref(kd)) == DST
