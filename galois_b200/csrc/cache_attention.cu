@@ -17,7 +17,7 @@ namespace {
 //  * The rows of all (sequence, key/value head) pairs form one list of 32-row blocks, which is dealt evenly to all
 //    warps of the device, each a contiguous part; a part may begin and end inside a pair.  No length is known on the
 //    host, and none makes a warp wait for another: a warp writes what it has of a pair as one piece (maximum, sum, HD
-//    numbers per head), and a second launch joins the pieces.
+//    means per head), and a second launch joins the pieces.
 //  * Each warp streams its blocks through a ring of its own in shared memory, across the borders of pairs: one TMA copy
 //    for the keys of a block and one for its values; nothing synchronises the CTA.  The logits of the next block are
 //    formed between the soft-max and the products of this one, so that a warp always has independent work to issue.
@@ -405,11 +405,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
                 if (t == 0) *reinterpret_cast<float2*>(p.stats + 2 * row) = make_float2(m, l);
                 // column 2 t of an n-tile stands for chunk t of a 128-byte row (column 2 t + 1 for chunk t + 4), or bytes 16 t (+ 8) of a 64-byte one
                 float* to = p.acc + row * HD + 16 * t;
+                const float mean = l == 0.0f ? 0.0f : vtop / l;  // as a mean: a sum of the largest values would leave f32's range
 #pragma unroll
                 for (int n = 0; n < NW; n++) {
                     const uint64_t* on = &o[n * 4];
-                    *reinterpret_cast<float4*>(to + 4 * n) = make_float4(low(on[0]) * vtop, low(on[1]) * vtop, low(on[2]) * vtop, low(on[3]) * vtop);
-                    *reinterpret_cast<float4*>(to + (HD == 128 ? 64 : 8) + 4 * n) = make_float4(high(on[0]) * vtop, high(on[1]) * vtop, high(on[2]) * vtop, high(on[3]) * vtop);
+                    *reinterpret_cast<float4*>(to + 4 * n) = make_float4(low(on[0]) * mean, low(on[1]) * mean, low(on[2]) * mean, low(on[3]) * mean);
+                    *reinterpret_cast<float4*>(to + (HD == 128 ? 64 : 8) + 4 * n) = make_float4(high(on[0]) * mean, high(on[1]) * mean, high(on[2]) * mean, high(on[3]) * mean);
                 }
             }
 #pragma unroll
@@ -478,27 +479,29 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const int32_t* __restri
         use = m == -INFINITY ? 0.0f : m;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            st[i].x = ex2(st[i].x - use);  // the piece's share
-            l += st[i].y * st[i].x;
+            st[i].y *= ex2(st[i].x - use);
+            l += st[i].y;
         }
         for (int i = lane + 128; i < n; i += 32) {
             const float2 s2 = *reinterpret_cast<const float2*>(stats + 2 * (row0 + (int64_t)i * rows));
             l += s2.y * ex2(s2.x - use);
         }
         l = gb_warp_sum(l);
+        const float by = l == 0.0f ? 0.0f : 1.0f / l;  // a piece's share of the result: its sum over all
         const float* a = acc + row0 * HD + lane * E;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             const int end = min(n, 32 * (k + 1));
 #pragma unroll 8
             for (int i = 32 * k + wr; i < end; i += W) {
-                const float f = __shfl_sync(0xffffffffu, st[k].x, i & 31);
+                const float f = __shfl_sync(0xffffffffu, st[k].y, i & 31) * by;
 #pragma unroll
                 for (int e = 0; e < E; e++) x[e] = fmaf(a[(int64_t)i * rows * HD + e], f, x[e]);
             }
         }
         for (int i = 128 + wr; i < n; i += W) {
-            const float f = ex2(stats[2 * (row0 + (int64_t)i * rows)] - use);
+            const float2 s2 = *reinterpret_cast<const float2*>(stats + 2 * (row0 + (int64_t)i * rows));
+            const float f = s2.y * ex2(s2.x - use) * by;
 #pragma unroll
             for (int e = 0; e < E; e++) x[e] = fmaf(a[(int64_t)i * rows * HD + e], f, x[e]);
         }
@@ -516,7 +519,7 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const int32_t* __restri
     }
     if (live && wr == 0) {
 #pragma unroll
-        for (int e = 0; e < E; e++) to[e] = l == 0.0f ? 0.0f : x[e] / l;
+        for (int e = 0; e < E; e++) to[e] = x[e];
         if (final_stats && lane == 0) *reinterpret_cast<float2*>(final_stats + 2 * ((int64_t)s * heads + head)) = make_float2(use, l);
     }
 }
@@ -531,7 +534,7 @@ __global__ void __launch_bounds__(256) cache_weights_kernel(const int32_t* __res
     for (int g = 0; g < group; g++) {
         const int64_t at = (int64_t)s * heads + kh * group + g;
         const float2 ml = *reinterpret_cast<const float2*>(stats + 2 * at);
-        x += ex2(scores[at * ctx + j] - ml.x) / ml.y;
+        if (ml.y != 0.0f) x += ex2(scores[at * ctx + j] - ml.x) / ml.y;
     }
     weights_out[kh * wo_head + s * wo_seq + j] = weights[kh * w_head + s * w_seq + j] + x;
 }
@@ -588,6 +591,7 @@ extern "C" int galois_b200_cache_attention_f32(galois_b200_ctx* ctx, const float
         return gb_fail(ctx, GALOIS_B200_E_SHAPE, "%s: q and dst must be {head_dim, heads, sequences} of the cache", what);
     if (heads > 65535 || (heads && (c.kv_heads == 0 || heads % c.kv_heads)))
         return gb_fail(ctx, GALOIS_B200_E_BROADCAST, "%s: %lld heads over %d key/value heads", what, (long long)heads, c.kv_heads);
+    if (!isfinite(scale)) return gb_fail(ctx, GALOIS_B200_E_BADARG, "%s: scale is not finite", what);
     if (heads == 0 || c.seqs == 0) return 0;
     if (!q || !lens || !dst || !workspace) return gb_fail(ctx, GALOIS_B200_E_BADARG, "%s: null pointer", what);
     if (qd->nb[0] != 1 || dd->nb[0] != 1 || (uintptr_t)q % 16 || (uintptr_t)dst % 16 || (heads > 1 && (qd->nb[1] % 4 || dd->nb[1] % 4)) ||

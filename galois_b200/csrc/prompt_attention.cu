@@ -520,6 +520,7 @@ int prompt_attention(galois_b200_ctx* ctx, const void* q, const galois_dim* qd, 
         return gb_fail(ctx, GALOIS_B200_E_SHAPE, "prompt_attention: q and dst, k and v must be of one shape each, all of one head_dim");
     const int heads = (int)qd->ne[1], kv_heads = (int)kd->ne[1], tq = (int)qd->ne[2], tk = (int)kd->ne[2];
     if (heads && (kv_heads == 0 || heads % kv_heads)) return gb_fail(ctx, GALOIS_B200_E_BROADCAST, "prompt_attention: %d heads over %d key/value heads", heads, kv_heads);
+    if (!isfinite(scale)) return gb_fail(ctx, GALOIS_B200_E_BADARG, "prompt_attention: scale is not finite");
     if (nseq < 0 || nseq > 0xfffff) return gb_fail(ctx, GALOIS_B200_E_BADARG, "prompt_attention: %d sequences", nseq);
     if (heads == 0 || tq == 0 || nseq == 0) return 0;
     if (!q_starts || !k_starts) return gb_fail(ctx, GALOIS_B200_E_BADARG, "prompt_attention: null pointer");
@@ -542,7 +543,7 @@ int prompt_attention(galois_b200_ctx* ctx, const void* q, const galois_dim* qd, 
     for (int i = 0; i < 3; i++) {
         // a tensor without tokens is not read; a dimension of one element has any stride
         const uint64_t size[3] = {(uint64_t)qd->ne[0], (uint64_t)std::max<int64_t>(1, dims[i]->ne[2]), (uint64_t)dims[i]->ne[1]};
-        const uint64_t stride[2] = {dims[i]->ne[2] > 1 ? (uint64_t)rows[i]->tok * 2 : 256, dims[i]->ne[1] > 1 ? (uint64_t)rows[i]->head * 2 : 256};
+        const uint64_t stride[2] = {dims[i]->ne[2] > 1 ? (uint64_t)rows[i]->tok * 2 : 256, dims[i]->ne[1] > 1 && dims[i]->ne[2] > 0 ? (uint64_t)rows[i]->head * 2 : 256};
         const uint32_t box[3] = {64, (uint32_t)(i == 0 ? PT : KT), 1};
         const void* base = dims[i]->ne[2] > 0 ? (const void*)rows[i]->p : q;
         rc = gb_tensor_map(ctx, maps + i, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, base, size, stride, box, 128);

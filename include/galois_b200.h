@@ -437,7 +437,8 @@ int galois_b200_decode_attention_f32(galois_b200_ctx* ctx, const galois_b200_dec
  * overlap operands except where stated.  Packed rows: tokens starts[s] <= t < starts[s + 1] of a {head_dim, heads,
  * tokens} tensor belong to sequence s (i32 on the device, nseq + 1 of them, ascending); rows behind the last
  * sequence are neither read nor written.  Starts, positions and lengths out of range: that sequence's part is left
- * out and the next synchronising call returns GALOIS_B200_E_BADARG. */
+ * out and the next synchronising call returns GALOIS_B200_E_BADARG.  `scale` is finite; logits that f32 cannot hold
+ * give what inf gives. */
 
 /* out_i = sum_j softmax_j(scale * q_i . k_j) v_j, where query i of a sequence with nq queries and nk keys sees the
  * keys j <= i + nk - nq (causal; a prompt that continues nk - nq earlier tokens).  Queries that see no key give

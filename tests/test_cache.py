@@ -866,3 +866,32 @@ def test_read_leaves_a_sequence_out_as_a_whole(dev, G, n):
     for out in outs:
         got = out.to_numpy()
         assert np.all(got[:n] == 9) and not np.any(got[n:] == 9)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_cache_attention_of_the_largest_values(dev, G, hd):
+    """The sum of many large values leaves f32's range, their mean does not."""
+    rng = np.random.default_rng(78)
+    lens = [3000, 33, 7]
+    kq, ks, vq, vs = random_cache(rng, 3, 1, 3000, hd)
+    vq[..., : hd // 2] = 120
+    vs[:] = np.float32(2.5e36)
+    q = rng.normal(0, 0.01, (3, 4, hd)).astype(np.float32)
+    out, bound, _, _ = R.step(q, kq, ks, vq, vs, lens, 0.125)
+    cache, dst = upload(G, (kq, ks, vq, vs)), put(G, np.zeros_like(q))
+    ws = gb.Tensor.zeros((gb.galois_cache_attention_workspace(cache, 4) // 4,), F32, G)
+    gb.galois_cache_attention(put(G, q), cache, put(G, np.array(lens, np.int32)), dst, 0.125, ws)
+    dev.synchronize()
+    assert np.all(np.abs(dst.to_numpy() - out) <= bound)
+
+
+def test_cache_attention_of_logits_below_the_range(dev, G):
+    """Every logit is -inf in f32: nothing counts, the result and the added weights are 0."""
+    kq, vq = np.full((1, 1, 40, 64), 127, np.int8), np.full((1, 1, 40, 64), 3, np.int8)
+    sc = np.full((1, 1, 2), 1e30, np.float32)
+    q, w = np.full((1, 2, 64), -1e30, np.float32), np.arange(40, dtype=np.float32).reshape(1, 1, 40)
+    cache, dst, wt = upload(G, (kq, sc, vq, np.ones_like(sc))), put(G, np.full_like(q, 5)), put(G, w)
+    ws = gb.Tensor.zeros((gb.galois_cache_attention_workspace(cache, 2, True) // 4,), F32, G)
+    gb.galois_cache_attention(put(G, q), cache, put(G, np.array([40], np.int32)), dst, 1.0, ws, weights=wt, weights_out=wt)
+    dev.synchronize()
+    assert not dst.to_numpy().any() and np.array_equal(wt.to_numpy(), w)

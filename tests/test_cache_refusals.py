@@ -179,3 +179,11 @@ def test_metadata_inside_what_is_written_is_refused(ctx):
     kd = rows()
     for a, b in ((1, 4), (3, 1), (2, 4), (3, 2)):  # starts, positions: in k, in k, in v, in v
         assert lib.galois_b200_cache_read_f32(ctx, C.byref(cache()), addr(a), addr(b), 3, addr(1), C.byref(kd), addr(2), C.byref(kd)) == DST
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf")])
+def test_a_scale_that_is_not_finite_is_refused(ctx, scale):
+    qd, kd, sd = dim((128, 4, 9)), dim((128, 2, 9)), dim((128, 4, 3))
+    for fn in (lib.galois_b200_prompt_attention_f16, lib.galois_b200_prompt_attention_f16_f32):
+        assert fn(ctx, addr(1), C.byref(qd), addr(2), C.byref(kd), addr(3), C.byref(kd), addr(4), addr(4), 2, addr(5), C.byref(qd), scale) == BADARG
+    assert lib.galois_b200_cache_attention_f32(ctx, addr(1), C.byref(sd), C.byref(cache()), addr(2), addr(3), C.byref(sd), scale, None, None, None, None, addr(5), 1 << 29) == BADARG
