@@ -29,9 +29,9 @@ namespace {
 //    for is chosen so that the eight lanes of a load's phase meet no bank of the swizzled tile twice.
 //
 // Measured (B200): 64 sequences of up to 8192 rows, 8 key/value heads x 128, groups of 4: 664 MB in 138 to 145 us, 4.6 to 4.8
-// TB/s, 0.70 to 0.74 of the copy rate; one sequence of 2048 rows, 32 heads: 13.9 us with the joining launch.  No unit is full (with twelve warps:
+// TB/s, 0.70 to 0.74 of the copy rate; one sequence of 2048 rows, 32 heads: 14.3 us with the joining launch.  No unit is full (with twelve warps:
 // issue 0.50, ALU 0.36, FMA 0.26, tensor cores 0.27): an MMA with the conversion of its operand takes 13 to 16 cycles of
-// a scheduler, the bare one 8.6.  Eight warps or twelve with shorter rings, in one run: the batch 145 and 141 us, one sequence
+// a scheduler, the bare one 8.6.  Eight warps or twelve with shorter rings, in one run (before pieces were kept as means): the batch 145 and 141 us, one sequence
 // 13.9 and 15.5, 16 sequences of up to 4096 with weights 37.7 and 38.5; eight lose 2.5 % on the first and gain on the others.
 constexpr int WARPS = 8;
 constexpr int BLK = GB_CACHE_BLOCK;
@@ -643,6 +643,7 @@ extern "C" int galois_b200_cache_attention_f32(galois_b200_ctx* ctx, const float
                                dim3(WARPS * 32), c.head_dim == 64 ? ring<64>::TOTAL : ring<128>::TOTAL, a, k_map, v_map));
         GB_LAUNCHED(ctx, what);
     }
+    // one sequence of 32 heads: 14.3 us with eight warps a head, 22.6 with one; 64 sequences of 32: 149.6 and 145.5
     const bool few = (int64_t)heads * c.seqs < 4 * ctx->sm_count;
     auto join = c.head_dim == 64 ? (few ? cache_join_kernel<64, 8> : cache_join_kernel<64, 1>) : (few ? cache_join_kernel<128, 8> : cache_join_kernel<128, 1>);
     GB_CUDA(ctx, gb_launch(ctx, join, dim3((unsigned)(few ? heads : (heads + 7) / 8), (unsigned)c.seqs), dim3(256), 0, lens, c.seqs, c.ctx, c.kv_heads, group,
