@@ -6,10 +6,12 @@
 // it grows the rows already held are brought to the new scale, q' = round(q d_held / d).  Both roundings are exact
 // (half to even), which makes the contents a function of the numbers alone, whatever the order or split of the calls'
 // work.  All move bytes and are meant to be bound by HBM (B200, 6.55 TB/s measured copy rate): 50 000 rows of 8 heads x 128
-// are read into F16 in 53 us (5.8 TB/s); 8 000 F16 tokens appended in 20 us (49 MB, 2.4 TB/s), held back by the instructions of
-// the rounding, 21 a number; 16 sequences of up to 8192 rows cut to 2048 in 43 us (134 MB of rows), some of it the
+// are read into F16 in 53 us (5.8 TB/s); 8 000 F16 tokens appended in 17.5 us (49 MB, 2.8 TB/s), held back by the instructions
+// of the rounding; 16 sequences of up to 8192 rows cut to 2048 in 43 us (134 MB of rows), some of it the
 // selection, whose passes over the digits wait for one another.  Few rows cost a launch.
 #include "kv_cache_q8.cuh"
+
+#include <type_traits>
 
 namespace {
 
@@ -121,28 +123,38 @@ __global__ void __launch_bounds__(128) cache_append_kernel(const T* __restrict__
         float d = fmaxf(__fdiv_rn(top, 127.0f), held);
         if (!(d >= Q8_TINY)) d = 0.0f;
         if (threadIdx.x == 0) *scale = d;
-        int8_t* to = q + s * c.seq + (int64_t)(block * GB_CACHE_BLOCK + row0) * c.tok;
-        const gb_around by = gb_make_around(d > 0.0f ? __fdiv_rn(1.0f, d) : 0.0f);
+        int8_t* const to = q + s * c.seq + (int64_t)(block * GB_CACHE_BLOCK + row0) * c.tok;
+        const gb_around by = gb_make_around(d > 0.0f ? __fdiv_rn(1.0f, d) : 0.0f);  // 0: everything becomes 0
+        auto store = [&](int i, const uint32_t(&w)[W]) {
+            if constexpr (W == 1) *reinterpret_cast<uint32_t*>(to + i * RPP * c.tok) = w[0];
+            else *reinterpret_cast<uint2*>(to + i * RPP * c.tok) = make_uint2(w[0], w[1]);
+        };
+        auto put = [&](auto with_odd) {
 #pragma unroll
-        for (int i = 0; i < N; i++, to += RPP * c.tok) {
-            const int row = row0 + i * RPP;
-            uint32_t w[W];
-            if (row >= lo && row < hi) {
+            for (int i = 0; i < N; i++) {
+                if (row0 + i * RPP < lo || row0 + i * RPP >= hi) continue;
+                uint32_t w[W];
 #pragma unroll
                 for (int j = 0; j < W; j++) {
                     float4 f = r[i].get(j);
-                    if (odd) f = make_float4(tame(f.x), tame(f.y), tame(f.z), tame(f.w));
-                    w[j] = d > 0.0f ? gb_q8_round4(f, d, by) : 0u;
+                    if constexpr (decltype(with_odd)::value) f = make_float4(tame(f.x), tame(f.y), tame(f.z), tame(f.w));
+                    w[j] = gb_q8_round4(f, d, by);
                 }
-            } else if (row < lo && d != held) {
-                const gb_around ratio = gb_make_around(d > 0.0f ? __fdiv_rn(held, d) : 0.0f);
-#pragma unroll
-                for (int j = 0; j < W; j++) w[j] = gb_q8_rescale4(reinterpret_cast<const uint32_t*>(to)[j], held, d, ratio);
-            } else {
-                continue;
+                store(i, w);
             }
-            if constexpr (W == 1) *reinterpret_cast<uint32_t*>(to) = w[0];
-            else *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+        };
+        if (odd) put(std::true_type());
+        else put(std::false_type());
+        if (lo > 0 && d != held) {  // the rows there are, to the larger scale
+            const gb_around ratio = gb_make_around(d > 0.0f ? __fdiv_rn(held, d) : 0.0f);
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                if (row0 + i * RPP >= lo) continue;
+                uint32_t w[W];
+#pragma unroll
+                for (int j = 0; j < W; j++) w[j] = gb_q8_rescale4(reinterpret_cast<const uint32_t*>(to + i * RPP * c.tok)[j], held, d, ratio);
+                store(i, w);
+            }
         }
         t = min(next, end);
     }
