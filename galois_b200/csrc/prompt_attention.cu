@@ -93,6 +93,7 @@ struct prompt_args {
     float scale;
     void* out;
     int64_t o_head, o_tok;
+    bool wide;  // rows of `out` begin at multiples of 32 bytes
     int* status;
 };
 
@@ -100,6 +101,21 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+__device__ __forceinline__ void store32(void* to, const uint32_t* x) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7]) : "memory");
+}
+// N words of a row.  32 bytes at a time fill a sector of memory, 16 half of one: results of 8192 tokens in 372 us and 379, of 2048 in
+// 52.8 and 53.3.
+template <int N>
+__device__ __forceinline__ void store_words(void* to, const uint32_t (&x)[N], bool wide) {
+    if (wide) {
+#pragma unroll
+        for (int e = 0; e < N / 8; e++) store32((uint4*)to + 2 * e, x + 8 * e);
+    } else {
+#pragma unroll
+        for (int e = 0; e < N / 4; e++) ((uint4*)to)[e] = make_uint4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+    }
 }
 // The largest, or NaN if one of them is: a logit that is not a number has to reach the result.
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -470,14 +486,12 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
                 if (!live) continue;
                 if constexpr (sizeof(T) == 4) {
-#pragma unroll
-                    for (int e = 0; e < 8; e++) reinterpret_cast<uint4*>(to)[i * 8 + e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                    store_words(reinterpret_cast<uint4*>(to) + i * 8, o, p.wide);
                 } else {
                     uint32_t h[16];
 #pragma unroll
                     for (int e = 0; e < 16; e++) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h[e]) : "f"(__uint_as_float(o[2 * e + 1])), "f"(__uint_as_float(o[2 * e])));
-#pragma unroll
-                    for (int e = 0; e < 4; e++) reinterpret_cast<uint4*>(to)[i * 4 + e] = make_uint4(h[4 * e], h[4 * e + 1], h[4 * e + 2], h[4 * e + 3]);
+                    store_words(reinterpret_cast<uint4*>(to) + i * 4, h, p.wide);
                 }
             }
             tc_before_sync();
@@ -536,7 +550,8 @@ int prompt_attention(galois_b200_ctx* ctx, const void* q, const galois_dim* qd, 
     // units as any lengths need, at most: each sequence has one tile at most that is not full
     const int64_t ctas = ((int64_t)tq / span + std::min(nseq, tq)) * units;
     if (ctas > 0x7fffffff) return gb_fail(ctx, GALOIS_B200_E_SHAPE, "prompt_attention: too many tokens");
-    const prompt_args a{qr, kr, vr, q_starts, k_starts, nseq, tq, tk, heads, group, scale, dst, dd->nb[1], dd->nb[2], ctx->dev_status};
+    const bool wide = (uintptr_t)dst % 32 == 0 && (heads == 1 || dd->nb[1] * sizeof(T) % 32 == 0) && (tq == 1 || dd->nb[2] * sizeof(T) % 32 == 0);
+    const prompt_args a{qr, kr, vr, q_starts, k_starts, nseq, tq, tk, heads, group, scale, dst, dd->nb[1], dd->nb[2], wide, ctx->dev_status};
     CUtensorMap maps[3];
     const rows16* rows[3] = {&qr, &kr, &vr};
     const galois_dim* dims[3] = {qd, kd, vd};

@@ -895,3 +895,17 @@ def test_cache_attention_of_logits_below_the_range(dev, G):
     gb.galois_cache_attention(put(G, q), cache, put(G, np.array([40], np.int32)), dst, 1.0, ws, weights=wt, weights_out=wt)
     dev.synchronize()
     assert not dst.to_numpy().any() and np.array_equal(wt.to_numpy(), w)
+
+
+@pytest.mark.parametrize("kind,pad", [(np.float32, 4), (np.float16, 8), (np.float32, 8), (np.float16, 16)])
+def test_prompt_attention_into_rows_of_any_alignment(dev, G, kind, pad):
+    """Rows of the destination begin at every 16 bytes, or every 32."""
+    rng = np.random.default_rng(79)
+    q, k, v, qs, ks = prompt_inputs(rng, 64, 3, 1, [(140, 150), (9, 9)], 1)
+    out, bound = R.prompt(q, k, v, qs, ks, 0.125)
+    bound = f16_bound(out, bound) if kind == np.float16 else bound
+    dst, _, _ = spread(G, np.full(q.shape, 3, kind), None, pad)
+    gb.galois_prompt_attention(put(G, q), put(G, k), put(G, v), put(G, qs), put(G, ks), dst, 0.125)
+    dev.synchronize()
+    got, n = back(dst, q.shape).astype(np.float64), qs[-1]
+    assert np.all(got[n:] == 3) and np.all(np.abs(got[:n] - out[:n]) <= bound[:n])
