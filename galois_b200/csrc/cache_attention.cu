@@ -28,8 +28,8 @@ namespace {
 //    the values, CW numbers of four rows, whose bytes are paired by permutes.  Which row and which chunk g and t stand
 //    for is chosen so that the eight lanes of a load's phase meet no bank of the swizzled tile twice.
 //
-// Measured (B200): 64 sequences of up to 8192 rows, 8 key/value heads x 128, groups of 4: 664 MB in 138 to 145 us, 4.6 to 4.8
-// TB/s, 0.70 to 0.74 of the copy rate; one sequence of 2048 rows, 32 heads: 14.3 us with the joining launch.  No unit is full (with twelve warps:
+// Measured (B200): 64 sequences of up to 8192 rows, 8 key/value heads x 128, groups of 4: 664 MB in 145 to 148 us, 4.5 TB/s,
+// 0.69 of the copy rate; one sequence of 2048 rows, 32 heads: 14.3 us with the joining launch.  No unit is full (with twelve warps:
 // issue 0.50, ALU 0.36, FMA 0.26, tensor cores 0.27): an MMA with the conversion of its operand takes 13 to 16 cycles of
 // a scheduler, the bare one 8.6.  Eight warps or twelve with shorter rings, in one run (before pieces were kept as means): the batch 145 and 141 us, one sequence
 // 13.9 and 15.5, 16 sequences of up to 4096 with weights 37.7 and 38.5; eight lose 2.5 % on the first and gain on the others.

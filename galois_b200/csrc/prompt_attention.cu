@@ -23,8 +23,8 @@
 // probabilities refer to is raised only when a row's maximum passes it by 2^8 (F16 holds what that leaves), so that the
 // results in tensor memory are rarely rescaled.
 //
-// Measured (B200): 8192 tokens in three prompts, 32 heads over 8 x 128: 369 to 380 us, 0.48 to 0.50 of the measured matrix rate;
-// 2048 tokens, 32 heads x 128: 51 to 53 us.  A step (two query tiles x 64 keys) takes some 1960 cycles: the products alone 1240
+// Measured (B200): 8192 tokens in three prompts, 32 heads over 8 x 128: 371 to 375 us, 0.49 of the measured matrix rate;
+// 2048 tokens, 32 heads x 128: 53 us.  A step (two query tiles x 64 keys) takes some 1960 cycles: the products alone 1240
 // of them (logits of 64 keys take 48 cycles an MMA, of 128 keys 64), the issuing warp's loop all of them, a tile's soft-max 1700.
 // Tiles of 128 keys with one buffer of logits and tiles of 64 with two, before values and keys shared slots: 378 and 383 us
 // on the first, 54.1 and 52.9 on the second, 10.2 and 8.8 on 300 tokens; 64 were taken for the shorter ones.  The shared slots: 375.
