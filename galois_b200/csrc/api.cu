@@ -338,13 +338,18 @@ extern "C" int galois_b200_htod(galois_b200_ctx* ctx, void* dst_dev, const void*
     gb_hazard_reset(ctx);
     return 0;
 }
+// What the device status says: kernels set it where a bounded wait runs out, and where what they read on the device (indices, starts,
+// positions, lengths) is out of range.
+static const char* status_text(int st) {
+    return st == GALOIS_B200_E_BADARG ? "an index, start, position or length on the device was out of range" : "a bounded device-side wait ran out";
+}
 static int check_dev_status(galois_b200_ctx* ctx) {
     int st = 0;
     GB_CUDA(ctx, cudaMemcpyAsync(&st, ctx->dev_status, sizeof(int), cudaMemcpyDeviceToHost, ctx->stream));
     GB_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
     if (st != 0) {
         GB_CUDA(ctx, cudaMemsetAsync(ctx->dev_status, 0, 256, ctx->stream));  // the status and the grid-barrier words behind it
-        return gb_fail(ctx, st, "a bounded device-side wait ran out (status %d)", st);
+        return gb_fail(ctx, st, "%s (status %d)", status_text(st), st);
     }
     return 0;
 }
@@ -409,7 +414,7 @@ extern "C" int galois_b200_dtoh_wait(galois_b200_ctx* ctx, int ticket) {
     const int st = ctx->d2h_status[ticket];
     if (st != 0) {
         // the status word stays set on the device until a synchronising call (galois_b200_synchronize, galois_b200_dtoh) clears it
-        return gb_fail(ctx, st, "a bounded device-side wait ran out in the work this read-back followed (status %d)", st);
+        return gb_fail(ctx, st, "%s in the work this read-back followed (status %d)", status_text(st), st);
     }
     return 0;
 }

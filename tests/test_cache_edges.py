@@ -1,0 +1,61 @@
+"""Prompt attention and the 8-bit cache where calls are at their edges: starts that are wrong, numbers at the end of f32, no heads, long
+evictions, operands that lie over one another, and the library's own mat-mul, rope and copy in front of them."""
+import numpy as np
+import pytest
+
+import cache_reference as R
+import galois_b200 as gb
+from galois_b200 import GError, GGmlType
+from test_cache import back, f16_bound, parts_of, prompt_inputs, put, random_cache, upload
+
+pytestmark = pytest.mark.gpu
+
+I8, I32, F16, F32 = GGmlType.I8, GGmlType.I32, GGmlType.F16, GGmlType.F32
+F32_MAX = np.finfo(np.float32).max
+
+
+@pytest.fixture()
+def G(dev):
+    return gb.Device.Gpu(dev)
+
+
+def reported(dev, text="out of range"):
+    with pytest.raises(GError) as e:
+        dev.synchronize()
+    assert e.value.code == -1 and text in str(e.value) and "wait" not in str(e.value), str(e.value)
+
+
+# ------------------------------------------------------------------------------------------------ starts and positions
+
+
+@pytest.mark.parametrize("what", ["append", "read", "prompt", "step", "evict"])
+def test_what_is_out_of_range_is_said_to_be(dev, G, what):
+    rng = np.random.default_rng(1)
+    cache = upload(G, random_cache(rng, 1, 1, 64, 64))
+    x, starts, pos = put(G, np.ones((5, 1, 64), np.float32)), put(G, np.array([0, 9], np.int32)), put(G, np.zeros(1, np.int32))
+    if what == "append":
+        gb.galois_cache_append(x, x, starts, pos, cache)
+    elif what == "read":
+        gb.galois_cache_read(cache, starts, pos, x, put(G, np.ones((5, 1, 64), np.float32)))
+    elif what == "prompt":
+        h = put(G, np.ones((5, 1, 64), np.float16))
+        gb.galois_prompt_attention(h, h, h, starts, starts, x, 0.1)
+    elif what == "step":
+        ws = gb.Tensor.zeros((gb.galois_cache_attention_workspace(cache, 1) // 4,), F32, G)
+        q = put(G, np.ones((1, 1, 64), np.float32))
+        gb.galois_cache_attention(q, cache, put(G, np.array([65], np.int32)), put(G, np.ones((1, 1, 64), np.float32)), 0.1, ws)
+    else:
+        cut = gb.CacheQ8.zeros(64, 32, 1, 1, G)
+        gb.galois_cache_evict(cache, put(G, np.array([65], np.int32)), put(G, np.ones((1, 1, 64), np.float32)), 4, cut, put(G, np.zeros(1, np.int32)),
+                              put(G, np.zeros((1, 1, 32), np.float32)), put(G, np.zeros((1, 1, 32), np.int32)))
+    reported(dev)
+    dev.synchronize()
+
+
+def descending(seqs, at, rng):
+    """Starts of `seqs` sequences of 3 to 70 tokens; those behind sequence `at` begin again from the front."""
+    lens = rng.integers(3, 71, seqs)
+    starts = R.starts_of(lens)
+    tokens = int(starts[-1])
+    starts[at + 1:] -= starts[at + 1] - 1
+    return starts.astype(np.int32), tokens
