@@ -22,8 +22,9 @@ namespace {
 //    for the keys of a block and one for its values; nothing synchronises the CTA.  The logits of the next block are
 //    formed between the soft-max and the products of this one, so that a warp always has independent work to issue.
 //  * The whole numbers are exact in F16, so both products run on mma.sync m16n8k16 with f32 sums: the 16 rows are up
-//    to 8 heads of the group twice, once with the upper and once with the lower 11 bits of the f32 operand (the query,
-//    scaled to 2^7..2^8; the probability), which keeps f32's accuracy.  The order of a contraction is free, so
+//    to 8 heads of the group twice, once with the upper and once with the lower 11 bits of the f32 operand.  The query is
+//    scaled to 2^14..2^15, a block's probabilities so that their largest is 2^15, and lower bits are kept times 2^12: numbers
+//    down to 2^-30 of the largest keep 22 bits, smaller ones are off by 2^-52 of it.  The order of a contraction is free, so
 //    fragments are taken as a lane's 16-byte loads give them: of the keys, lane (g, t) has numbers 16 t.. of one row; of
 //    the values, CW numbers of four rows, whose bytes are paired by permutes.  Which row and which chunk g and t stand
 //    for is chosen so that the eight lanes of a load's phase meet no bank of the swizzled tile twice.
@@ -48,11 +49,6 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
 __device__ __forceinline__ float low(uint64_t a) { return __uint_as_float((uint32_t)a); }
 __device__ __forceinline__ float high(uint64_t a) { return __uint_as_float((uint32_t)(a >> 32)); }
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
@@ -60,11 +56,13 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
     return d;
 }
-// Two numbers as F16 pairs: the nearest, and what is left of each.
+// Two numbers, at most 2^15, as F16 pairs: the nearest, and what is left of each (at most 2^3) times 2^12.  Without that factor the
+// lower halves of numbers below 2^-3 would fall below F16's normal range.
+constexpr float LOW = 0x1p-12f;
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
     hi = pack_half2(a, b);
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-    lo = pack_half2(a - f.x, b - f.y);
+    lo = pack_half2((a - f.x) * (1.0f / LOW), (b - f.y) * (1.0f / LOW));
 }
 __device__ __forceinline__ uint32_t minus_1152(uint32_t h) {  // 1024 + (q + 128) -> q, exact
     const __half2 r = __hadd2(*reinterpret_cast<const __half2*>(&h), __half2half2(__ushort_as_half((unsigned short)0xe480)));
@@ -247,7 +245,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     bool live = false;       // this lane's head exists
     float* scores = nullptr;  // its logits' row, where they are wanted
     // The query of the pair at `at`: lane (g, t) holds numbers 16 (t + 4 i) + 4 j.. of head g, times the power of two that
-    // brings the largest to 2^7..2^8, as two F16 each.
+    // brings the largest to 2^14..2^15, as two F16 each.
     auto load_query = [&]() {
         const int head = at.kh * p.group + at.tile * 8 + g;
         live = g < p.group - at.tile * 8;
@@ -263,8 +261,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const int e = max(-110, min(120, (int)(__float_as_uint(top) >> 23) - 127));
-        const float up = __uint_as_float((uint32_t)(127 + 7 - e) << 23);
-        factor = __uint_as_float((uint32_t)(127 - 7 + e) << 23) * p.scale * 1.4426950408889634f;
+        const float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+        factor = __uint_as_float((uint32_t)(127 - 14 + e) << 23) * p.scale * 1.4426950408889634f;
 #pragma unroll
         for (int i = 0; i < KS; i++) {
             split2(f[i].x * up, f[i].y * up, qa[i][0], qa[i][1]);
@@ -292,9 +290,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
             }
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                float y = s[0][e] + s[0][e + 2];
-                if constexpr (KS == 8) y += s[1][e] + s[1][e + 2];
-                x[j][e] = y * f;
+                float hi = s[0][e], lo = s[0][e + 2];
+                if constexpr (KS == 8) hi += s[1][e], lo += s[1][e + 2];
+                x[j][e] = fmaf(lo, LOW, hi) * f;
             }
         }
     };
@@ -302,7 +300,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     uint64_t o[NW * 4];  // pairs of f32
 #pragma unroll
     for (int i = 0; i < NW * 4; i++) o[i] = 0;
-    float m = -INFINITY, l = 0.0f, vinv = 0.0f, vtop = 0.0f;
+    // `l`, the sum of the piece's probabilities, is in units of 2^m, `o` in units of 2^(o_ref + o_exp).  Both are raised when a block passes
+    // them by more than 2^SLACK, which f32 has room for, so that sums are rarely rescaled.
+    constexpr float SLACK = 8.0f;
+    float m = -INFINITY, l = 0.0f, o_ref = -INFINITY;
+    int o_exp = 0;
     float x[4][2], xn[4][2];
     load_query();
     int slot = 0;
@@ -335,27 +337,36 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
         float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1])), fmaxf(fmaxf(x[2][0], x[2][1]), fmaxf(x[3][0], x[3][1])));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const float m1 = fmaxf(m, top), use = m1 == -INFINITY ? 0.0f : m1, v_scale = scales[0].y;
-        // the values' scales are taken relative to a power of two above the largest so far, so that their product with a
-        // probability keeps 22 bits in two F16
-        const float vt = __uint_as_float(max(__float_as_uint(v_scale) & 0x7f800000u, 0x0d800000u) + 0x00800000u);  // 2^k > v_scale, at least 2^-99
-        if (__any_sync(0xffffffffu, m1 > m || vt > vtop)) {
-            const float keep = ex2(m - use);
-            const float vt1 = fmaxf(vt, vtop), vinv1 = __uint_as_float((254u << 23) - __float_as_uint(vt1)), keep_o = keep * (vtop * vinv1);
-            l *= keep;
+        const float ref = top == -INFINITY ? 0.0f : top, v_scale = scales[0].y;
+        // v_scale = v_part 2^v_exp, 1/2 <= |v_part| < 1 (or what 0, the smallest numbers and NaN leave)
+        const uint32_t v_bits = __float_as_uint(v_scale);
+        const int v_exp = (int)((v_bits >> 23) & 255u) - 126;
+        const float v_part = (uint32_t)(v_exp + 125) < 254u ? __uint_as_float((v_bits & 0x807fffffu) | 0x3f000000u) : v_scale * 0x1p126f;
+        // Results are summed in units of the largest probability x value scale there was: a block whose values are loud counts
+        // only as far as its probabilities do.
+        float rise = (top - o_ref) + (float)(v_exp - o_exp);  // log2 of the block's unit over that of `o`
+        const bool higher = top > -INFINITY && !(rise <= SLACK), louder = top > m + SLACK;  // also the first finite logit
+        if (__any_sync(0xffffffffu, louder || higher)) {
+            const float keep_o = higher ? ex2(-rise) : 1.0f;
 #pragma unroll
             for (int i = 0; i < NW * 4; i++) o[i] = f2_mul(o[i], f2_pack(keep_o, keep_o));
-            m = m1, vtop = vt1, vinv = vinv1;
+            if (higher) o_ref = top, o_exp = v_exp, rise = 0.0f;
+            if (louder) l *= ex2(m - top), m = top;
         }
-        const float vr = v_scale * vinv;
-        // rows of a last block that lie behind the length have probability 0, and whole numbers as values, whatever they are
+        // what the block's sums count in the piece: of values, of probabilities
+        const float vw = top == -INFINITY ? 0.0f : ex2(rise) * v_part, lw = top == -INFINITY ? 0.0f : ex2(top - m);
+        // Probabilities are relative to the block's largest, so that F16 halves hold its small ones beside it.  Rows of a last
+        // block that lie behind the length have probability 0, and whole numbers as values, whatever they are.
         uint32_t ph[4], pl[4];
+        float sum = 0.0f;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const float p0 = ex2(x[j][0] - use), p1 = ex2(x[j][1] - use);
-            l += p0 + p1;
-            split2(p0 * vr, p1 * vr, ph[j], pl[j]);
+            const float p0 = ex2(x[j][0] - ref), p1 = ex2(x[j][1] - ref);
+            sum += p0 + p1;
+            split2(p0 * 0x1p15f, p1 * 0x1p15f, ph[j], pl[j]);
         }
+        l = fmaf(sum, lw, l);
+        const uint64_t w_hi = f2_pack(vw * 0x1p-15f, vw * 0x1p-15f), w_lo = f2_pack(vw * (0x1p-15f * LOW), vw * (0x1p-15f * LOW));
         uint32_t r[2][4][NW];  // [half of the block][row][word]
 #pragma unroll
         for (int h = 0; h < 2; h++)
@@ -371,7 +382,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
                 }
             }
         // The tensor cores cut their sums off instead of rounding them, which over thousands of rows would add up to one
-        // side: a block's sum is formed there and added to the running one by an ordinary addition.
+        // side: a block's sum is formed there and added to the running one by ordinary additions.
 #pragma unroll
         for (int n = 0; n < NW; n++) {
             float y[4][4];
@@ -389,7 +400,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
                 }
             }
 #pragma unroll
-            for (int j = 0; j < 4; j++) o[n * 4 + j] = add2(o[n * 4 + j], add2(f2_pack(y[j][0], y[j][1]), f2_pack(y[j][2], y[j][3])));
+            for (int j = 0; j < 4; j++) o[n * 4 + j] = f2_fma(f2_pack(y[j][2], y[j][3]), w_lo, f2_fma(f2_pack(y[j][0], y[j][1]), w_hi, o[n * 4 + j]));
         }
         __syncwarp();
         if (more) fetch_values(slot);
@@ -405,17 +416,22 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
                 if (t == 0) *reinterpret_cast<float2*>(p.stats + 2 * row) = make_float2(m, l);
                 // column 2 t of an n-tile stands for chunk t of a 128-byte row (column 2 t + 1 for chunk t + 4), or bytes 16 t (+ 8) of a 64-byte one
                 float* to = p.acc + row * HD + 16 * t;
-                const float mean = l == 0.0f ? 0.0f : vtop / l;  // as a mean: a sum of the largest values would leave f32's range
+                // as means: a sum of the largest values would leave f32's range, and so may the unit of `o`, in two factors therefore
+                const float unit = (o_ref - m) + (float)o_exp, far = unit > 0.0f ? 0x1p16f : 1.0f;
+                const float mean = l == 0.0f ? 0.0f : ex2(unit > 0.0f ? unit - 16.0f : unit) / l;
+                const uint64_t by = f2_pack(mean, mean), by2 = f2_pack(far, far);
 #pragma unroll
                 for (int n = 0; n < NW; n++) {
-                    const uint64_t* on = &o[n * 4];
-                    *reinterpret_cast<float4*>(to + 4 * n) = make_float4(low(on[0]) * mean, low(on[1]) * mean, low(on[2]) * mean, low(on[3]) * mean);
-                    *reinterpret_cast<float4*>(to + (HD == 128 ? 64 : 8) + 4 * n) = make_float4(high(on[0]) * mean, high(on[1]) * mean, high(on[2]) * mean, high(on[3]) * mean);
+                    uint64_t on[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) on[e] = f2_mul(f2_mul(o[n * 4 + e], by), by2);
+                    *reinterpret_cast<float4*>(to + 4 * n) = make_float4(low(on[0]), low(on[1]), low(on[2]), low(on[3]));
+                    *reinterpret_cast<float4*>(to + (HD == 128 ? 64 : 8) + 4 * n) = make_float4(high(on[0]), high(on[1]), high(on[2]), high(on[3]));
                 }
             }
 #pragma unroll
             for (int i = 0; i < NW * 4; i++) o[i] = 0;
-            m = -INFINITY, l = 0.0f, vtop = 0.0f, vinv = 0.0f;
+            m = -INFINITY, l = 0.0f, o_ref = -INFINITY, o_exp = 0;
             if (todo > 1) {
                 load_query();
                 logits(next, scales[0].x, xn);
