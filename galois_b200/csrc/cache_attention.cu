@@ -9,6 +9,8 @@
 #include "ptx.cuh"
 #include "tma.cuh"
 
+#include <math.h>
+
 namespace {
 
 // What has to be read is 2 HD bytes a row and head (the arithmetic, 4 HD flops a row and query head, is far below
@@ -58,7 +60,7 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
 }
 // Two numbers, at most 2^15, as F16 pairs: the nearest, and what is left of each (at most 2^3) times 2^12.  Without that factor the
 // lower halves of numbers below 2^-3 would fall below F16's normal range.
-constexpr float LOW = 0x1p-12f;
+constexpr float LOW = 0x1p-12f, F32_MAX = 3.402823466e38f;
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
     hi = pack_half2(a, b);
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
@@ -144,7 +146,8 @@ struct step_args {
     const int32_t* lens;
     int group, tiles;  // query heads per key/value head; tiles of 8 of them
     int rows;          // min(8, group): heads that a piece holds
-    float scale;
+    float scale;       // scale * log2(e) / 2^scale_exp, 1/2 to 1
+    int scale_exp;
     float *acc, *stats;  // pieces: [piece][rows][HD], [piece][rows][2]
     float* scores;       // [seq][heads][ctx] base-2 logits, or null
     int* status;
@@ -241,7 +244,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     };
 
     uint32_t qa[KS][4];
-    float factor = 0.0f;
+    float factor = 0.0f, factor2 = 0.0f;  // their product turns a key scale into the base-2 logit of a product of whole numbers
     bool live = false;       // this lane's head exists
     float* scores = nullptr;  // its logits' row, where they are wanted
     // The query of the pair at `at`: lane (g, t) holds numbers 16 (t + 4 i) + 4 j.. of head g, times the power of two that
@@ -260,9 +263,13 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int e = max(-110, min(120, (int)(__float_as_uint(top) >> 23) - 127));
+        const int e = max(-110, (int)(__float_as_uint(top) >> 23) - 127);
         const float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
-        factor = __uint_as_float((uint32_t)(127 - 14 + e) << 23) * p.scale * 1.4426950408889634f;
+        // The scale, the query's power of two and the key's scale may each be near an end of f32's range, and only their product an
+        // ordinary number: the powers of two come in as two halves, so that nothing is lost unless the product itself is.
+        const int pow2 = max(-252, e - 14 + p.scale_exp), half = pow2 >> 1;
+        factor = p.scale * __uint_as_float((uint32_t)(127 + half) << 23);
+        factor2 = __uint_as_float((uint32_t)(127 + pow2 - half) << 23);
 #pragma unroll
         for (int i = 0; i < KS; i++) {
             split2(f[i].x * up, f[i].y * up, qa[i][0], qa[i][1]);
@@ -272,7 +279,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     // Base-2 logits of a block's 32 rows: lane (g, t) gets those of head g and rows row_of(j, 2 t), row_of(j, 2 t + 1).
     auto logits = [&](int slot, float k_scale, float (&x)[4][2]) {
         const uint32_t ks = base + (uint32_t)(slot * ring<HD>::HALF);
-        const float f = k_scale * factor;
+        float f = k_scale * factor * factor2;
+        if (fabsf(f) > F32_MAX) f = copysignf(F32_MAX, f);  // a product of 0 is a logit of 0 all the same
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             float s[KS / 4][4];
@@ -654,7 +662,9 @@ extern "C" int galois_b200_cache_attention_f32(galois_b200_ctx* ctx, const float
         int r = gb_tensor_map(ctx, &k_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, c.k, size, stride, box, c.head_dim);
         if (r == 0) r = gb_tensor_map(ctx, &v_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, c.v, size, stride, box, c.head_dim);
         if (r) return r;
-        const step_args a{q, qd->nb[1], qd->nb[2], c, lens, group, tiles, rows, scale, ws + L.acc, ws + L.stats, scores, ctx->dev_status};
+        int scale_exp = 0;
+        const double part = frexp((double)scale * 1.4426950408889634, &scale_exp);
+        const step_args a{q, qd->nb[1], qd->nb[2], c, lens, group, tiles, rows, (float)part, scale_exp, ws + L.acc, ws + L.stats, scores, ctx->dev_status};
         GB_CUDA(ctx, gb_launch(ctx, c.head_dim == 64 ? cache_attention_kernel<64> : cache_attention_kernel<128>, dim3((unsigned)ctx->sm_count),
                                dim3(WARPS * 32), c.head_dim == 64 ? ring<64>::TOTAL : ring<128>::TOTAL, a, k_map, v_map));
         GB_LAUNCHED(ctx, what);

@@ -168,3 +168,30 @@ def test_a_loud_channel_of_the_query_that_no_key_has(dev, G, hd):
     ks, vs = np.ones((1, 1, 7), np.float32), np.full((1, 1, 7), 0.02, np.float32)
     out, tol = step64(q, kq, ks, vq, vs, [n], 2.0**-6)
     close(attend(dev, G, q, (kq, ks, vq, vs), [n], 2.0**-6), out, tol)
+
+
+def test_a_factor_below_the_range_of_f32(dev, G):
+    """Small queries, a small scale, large keys: only their product is an ordinary number."""
+    rng = np.random.default_rng(7)
+    n, hd = 100, 64
+    q = (rng.integers(-(2**14) + 1, 2**14, (1, 3, hd)) * 2.0**-119).astype(np.float32)
+    kq = rng.integers(-7, 8, (1, 1, n, hd)).astype(np.int8)
+    vq = rng.integers(1, 128, (1, 1, n, hd)).astype(np.int8)
+    ks, vs = np.full((1, 1, 4), 2.0**120, np.float32), np.full((1, 1, 4), 0.02, np.float32)
+    out, tol = step64(q, kq, ks, vq, vs, [n], 2.0**-17)
+    assert tol.max() < 1e-3 * out.min()
+    close(attend(dev, G, q, (kq, ks, vq, vs), [n], 2.0**-17), out, tol)
+
+
+def test_keys_of_zeros_under_a_factor_beyond_the_range_of_f32(dev, G):
+    """A logit of 0 stays 0 beside others that f32 does not hold."""
+    n, hd = 100, 64
+    rng = np.random.default_rng(8)
+    q = np.full((1, 2, hd), -(2.0**127), np.float32)
+    kq = np.zeros((1, 1, n, hd), np.int8)
+    kq[0, 0, ::2] = 5
+    vq = rng.integers(1, 128, (1, 1, n, hd)).astype(np.int8)
+    ks, vs = np.full((1, 1, 4), 2.0**20, np.float32), np.full((1, 1, 4), 0.02, np.float32)
+    got = attend(dev, G, q, (kq, ks, vq, vs), [n], 1.0)
+    want = (vq[0, 0, 1::2].astype(np.float64) * np.float64(vs[0, 0, 0])).mean(0)
+    assert np.all(np.abs(got - want) <= 2.0**-16 * want)  # as step64 counts, without logits
