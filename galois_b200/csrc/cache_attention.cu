@@ -19,7 +19,7 @@ namespace {
 //  * The rows of all (sequence, key/value head) pairs form one list of 32-row blocks, which is dealt evenly to all
 //    warps of the device, each a contiguous part; a part may begin and end inside a pair.  No length is known on the
 //    host, and none makes a warp wait for another: a warp writes what it has of a pair as one piece (maximum, sum, HD
-//    means per head), and a second launch joins the pieces.
+//    halved means per head), and a second launch joins the pieces.
 //  * Each warp streams its blocks through a ring of its own in shared memory, across the borders of pairs: one TMA copy
 //    for the keys of a block and one for its values; nothing synchronises the CTA.  The logits of the next block are
 //    formed between the soft-max and the products of this one, so that a warp always has independent work to issue.
@@ -424,8 +424,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
                 if (t == 0) *reinterpret_cast<float2*>(p.stats + 2 * row) = make_float2(m, l);
                 // column 2 t of an n-tile stands for chunk t of a 128-byte row (column 2 t + 1 for chunk t + 4), or bytes 16 t (+ 8) of a 64-byte one
                 float* to = p.acc + row * HD + 16 * t;
-                // as means: a sum of the largest values would leave f32's range, and so may the unit of `o`, in two factors therefore
-                const float unit = (o_ref - m) + (float)o_exp, far = unit > 0.0f ? 0x1p16f : 1.0f;
+                // As means: a sum of the largest values would leave f32's range, and so may the unit of `o`, in two factors therefore.  As
+                // half of them: 127 times the largest scale that append makes is rounded to infinity, which no share of 0 would hide.
+                const float unit = (o_ref - m) + (float)o_exp, far = unit > 0.0f ? 0x1p15f : 0.5f;
                 const float mean = l == 0.0f ? 0.0f : ex2(unit > 0.0f ? unit - 16.0f : unit) / l;
                 const uint64_t by = f2_pack(mean, mean), by2 = f2_pack(far, far);
 #pragma unroll
@@ -543,7 +544,10 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const int32_t* __restri
     }
     if (live && wr == 0) {
 #pragma unroll
-        for (int e = 0; e < E; e++) to[e] = x[e];
+        for (int e = 0; e < E; e++) {  // pieces hold half of their means; what that takes beyond f32 was stored as its largest number
+            const float y = 2.0f * x[e];
+            to[e] = fabsf(y) > F32_MAX ? copysignf(F32_MAX, y) : y;
+        }
         if (final_stats && lane == 0) *reinterpret_cast<float2*>(final_stats + 2 * ((int64_t)s * heads + head)) = make_float2(use, l);
     }
 }

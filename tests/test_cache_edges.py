@@ -59,3 +59,33 @@ def descending(seqs, at, rng):
     tokens = int(starts[-1])
     starts[at + 1:] -= starts[at + 1] - 1
     return starts.astype(np.int32), tokens
+
+
+# ------------------------------------------------------------------------------------------------ numbers at the end of f32
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_cache_attention_over_infinite_values(dev, G, hd):
+    """A row that alone counts gives the largest number; one that does not count gives nothing, not NaN."""
+    rng = np.random.default_rng(3)
+    ctx = 96
+    x = rng.normal(0, 1, (3, ctx, hd)).astype(np.float32)
+    x[0, 0, ::2], x[0, 0, 1::2] = np.inf, -np.inf
+    x[1, 5], x[2, 40] = np.inf, -np.inf
+    k = np.zeros((3, ctx, hd), np.float32)
+    k[1, :32, 0], k[2, 32:64, 0] = -127, -127  # the whole block, as its other rows are zeros now
+    cache = gb.CacheQ8.zeros(hd, ctx, 1, 3, G)
+    starts = put(G, np.arange(4, dtype=np.int32) * ctx)
+    gb.galois_cache_append(put(G, k.reshape(-1, 1, hd)), put(G, x.reshape(-1, 1, hd)), starts, put(G, np.zeros(3, np.int32)), cache)
+    q = np.zeros((3, 2, hd), np.float32)
+    q[..., 0] = 8
+    dst = put(G, np.zeros_like(q))
+    ws = gb.Tensor.zeros((gb.galois_cache_attention_workspace(cache, 2) // 4,), F32, G)
+    gb.galois_cache_attention(put(G, q), cache, put(G, np.array([1, ctx, ctx], np.int32)), dst, 1.0, ws)
+    dev.synchronize()
+    got = dst.to_numpy().astype(np.float64)
+    assert np.all(got[0, :, ::2] == F32_MAX) and np.all(got[0, :, 1::2] == -F32_MAX)
+    for s, gone in ((1, slice(0, 32)), (2, slice(32, 64))):
+        rows = np.delete(x[s].astype(np.float64), np.r_[gone], axis=0)
+        step = np.abs(rows).max() / 127 / 2  # what the 8 bits are off by, at most
+        assert np.all(np.abs(got[s] - rows.mean(0)) <= step * 1.001)
