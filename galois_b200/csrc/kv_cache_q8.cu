@@ -17,8 +17,11 @@ namespace {
 
 constexpr float Q8_TINY = 0x1p-100f;  // a smaller scale stands for a block of zeros (its quotients could underflow)
 constexpr float Q8_MAX = 3.402823466e38f;
+// 127 times a larger scale is rounded to infinity.  Append makes one such scale, f32(Q8_MAX / 127), for what it stores as Q8_MAX.
+constexpr float Q8_SAFE = 0x1.020406p+121f;
 
-__device__ __forceinline__ float tame(float x) { return x != x ? 0.0f : fminf(fmaxf(x, -Q8_MAX), Q8_MAX); }
+__device__ __forceinline__ float finite(float x) { return fminf(fmaxf(x, -Q8_MAX), Q8_MAX); }
+__device__ __forceinline__ float tame(float x) { return x != x ? 0.0f : finite(x); }
 
 // 16 bytes of a row of new numbers: 4 f32 or 8 F16.
 template <typename T>
@@ -240,6 +243,20 @@ __global__ void __launch_bounds__(128) cache_read_kernel(gb_cache_view c, const 
         } else {
             __half2 h[4] = {__floats2half2_rn(f[0].x, f[0].y), __floats2half2_rn(f[0].z, f[0].w), __floats2half2_rn(f[W - 1].x, f[W - 1].y), __floats2half2_rn(f[W - 1].z, f[W - 1].w)};
             *reinterpret_cast<uint4*>(to) = *reinterpret_cast<uint4*>(h);
+        }
+    }
+    if constexpr (sizeof(T) == 4) {
+        bool loud = false;
+#pragma unroll
+        for (int i = 0; i < N; i++) loud = loud || (live[i] && d[i] > Q8_SAFE);
+        if (loud) {  // once more, for the rows that hold f32's largest number
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                if (!live[i] || !(d[i] > Q8_SAFE)) continue;
+                const float4 f = gb_q8_float4(w[i][0]);
+                *reinterpret_cast<float4*>(y + (int64_t)(t0 + i * RPP) * y_tok) =
+                    make_float4(finite(__fmul_rn(f.x, d[i])), finite(__fmul_rn(f.y, d[i])), finite(__fmul_rn(f.z, d[i])), finite(__fmul_rn(f.w, d[i])));
+            }
         }
     }
 }

@@ -466,14 +466,15 @@ typedef struct galois_b200_cache_q8 {
  * cache row pos[s] + i of slot s.  A block of 32 rows has the scale f32(max |x| / 127) of the largest number it was
  * given; if the block already holds rows before pos[s] and the scale has to grow, they are brought to the new one.
  * Numbers are rounded half to even from the exact quotient x / scale.  NaN is stored as 0, infinities as the largest
- * finite number; a scale below 2^-100 as 0, and its block as zeros.  Rows at and behind pos[s] that the block held
+ * finite f32; a scale below 2^-100 as 0, and its block as zeros.  Rows at and behind pos[s] that the block held
  * before do not count. */
 int galois_b200_cache_append_f32(galois_b200_ctx* ctx, const galois_b200_cache_q8* cache, const float* k, const galois_dim* kd, const float* v,
                                  const galois_dim* vd, const int32_t* starts, const int32_t* pos, int nseq);
 int galois_b200_cache_append_f16(galois_b200_ctx* ctx, const galois_b200_cache_q8* cache, const void* k, const galois_dim* kd, const void* v,
                                  const galois_dim* vd, const int32_t* starts, const int32_t* pos, int nseq);
-/* The inverse: packed row i of sequence s of k and v receives the values of cache row pos[s] + i of slot s (exact in
- * f32, rounded to nearest even in F16), e.g. the earlier tokens that a prompt continues. */
+/* The inverse: packed row i of sequence s of k and v receives the values of cache row pos[s] + i of slot s, e.g. the earlier
+ * tokens that a prompt continues.  A value is the product of number and scale, rounded half to even to f32 (what append
+ * stored as the largest finite number comes back as that) and, for the F16 form, from there to F16. */
 int galois_b200_cache_read_f32(galois_b200_ctx* ctx, const galois_b200_cache_q8* cache, const int32_t* starts, const int32_t* pos, int nseq,
                                float* k, const galois_dim* kd, float* v, const galois_dim* vd);
 int galois_b200_cache_read_f16(galois_b200_ctx* ctx, const galois_b200_cache_q8* cache, const int32_t* starts, const int32_t* pos, int nseq,

@@ -64,6 +64,29 @@ def descending(seqs, at, rng):
 # ------------------------------------------------------------------------------------------------ numbers at the end of f32
 
 
+def test_infinities_come_back_as_the_largest_number(dev, G):
+    """127 times the scale f32(largest / 127) is beyond f32; what was stored as the largest finite number is read as that."""
+    x = np.zeros((40, 1, 64), np.float32)
+    x[0, 0, :4] = [np.inf, -np.inf, F32_MAX, -F32_MAX]
+    x[35, 0, :3] = [3e38, -3e38, 1]
+    cache = gb.CacheQ8.zeros(64, 64, 1, 1, G)
+    s, p = put(G, np.array([0, 40], np.int32)), put(G, np.zeros(1, np.int32))
+    gb.galois_cache_append(put(G, x), put(G, -x), s, p, cache)
+    outs = [put(G, np.full(x.shape, 9, np.float32)) for _ in range(2)]
+    gb.galois_cache_read(cache, s, p, *outs)
+    dev.synchronize()
+    want = np.clip(x.astype(np.float64), -F32_MAX, F32_MAX)
+    for sign, out in zip((1, -1), outs):
+        got = out.to_numpy().astype(np.float64) * sign
+        assert np.all(np.isfinite(got))
+        assert np.array_equal(got[0], want[0]) and not got[1:32].any()
+        assert np.all(np.abs(got[35] - want[35]) <= 3e38 / 127 * 0.5000001)
+    half = [put(G, np.full(x.shape, 9, np.float16)) for _ in range(2)]
+    gb.galois_cache_read(cache, s, p, *half)
+    dev.synchronize()
+    assert list(half[0].to_numpy()[0, 0, :4]) == [np.inf, -np.inf, np.inf, -np.inf]  # what F16 makes of them
+
+
 @pytest.mark.parametrize("hd", [64, 128])
 def test_cache_attention_over_infinite_values(dev, G, hd):
     """A row that alone counts gives the largest number; one that does not count gives nothing, not NaN."""
