@@ -97,6 +97,11 @@ __device__ __forceinline__ int row_of(int j, int n) {
 }
 
 __device__ __forceinline__ int checked_len(int n, int ctx) { return n < 0 || n > ctx ? 0 : n; }
+// By one warp of the first kernel that a call launches.
+__device__ __forceinline__ void report_lens(const int32_t* __restrict__ lens, int n, int ctx, int* __restrict__ status) {
+    for (int i = threadIdx.x & 31; i < n; i += 32)
+        if (lens[i] < 0 || lens[i] > ctx) *status = GALOIS_B200_E_BADARG;
+}
 
 // How the list of blocks is dealt: `total` blocks over `warps` contiguous parts, none of them empty.
 struct deal {
@@ -172,9 +177,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     const gb_cache_view& c = p.c;
     const int per = c.kv_heads * p.tiles, heads = c.kv_heads * p.group;
     const deal D(count_blocks(p.lens, c.seqs, c.ctx, per), (int)gridDim.x * WARPS);
-    if (blockIdx.x == 0 && warp == 0)
-        for (int i = lane; i < c.seqs; i += 32)
-            if (p.lens[i] < 0 || p.lens[i] > c.ctx) *p.status = GALOIS_B200_E_BADARG;
+    if (blockIdx.x == 0 && warp == 0) report_lens(p.lens, c.seqs, c.ctx, p.status);
     const int w = warp * (int)gridDim.x + (int)blockIdx.x;  // parts of neighbours lie on different SMs
     if (w >= D.warps) return;
     const int64_t b0 = D.begin(w);
@@ -463,8 +466,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
 template <int HD, int W>
 __global__ void __launch_bounds__(256) cache_join_kernel(const int32_t* __restrict__ lens, int nseq, int ctx, int kv_heads, int group, int tiles, int rows,
                                                          int warps, const float* __restrict__ acc, const float* __restrict__ stats,
-                                                         float* __restrict__ out, int64_t o_head, int64_t o_seq, float* __restrict__ final_stats) {
+                                                         float* __restrict__ out, int64_t o_head, int64_t o_seq, float* __restrict__ final_stats,
+                                                         int* __restrict__ status) {
     gb_pdl_entry();
+    if (ctx == 0 && blockIdx.x + blockIdx.y == 0 && threadIdx.x < 32) report_lens(lens, nseq, ctx, status);
     constexpr int E = HD / 32, PER_CTA = 8 / W;
     __shared__ float part[8][HD];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wr = warp % W;
@@ -554,8 +559,9 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const int32_t* __restri
 
 __global__ void __launch_bounds__(256) cache_weights_kernel(const int32_t* __restrict__ lens, const float* __restrict__ stats, const float* __restrict__ scores,
                                                             const float* weights, int64_t w_head, int64_t w_seq, float* weights_out, int64_t wo_head,
-                                                            int64_t wo_seq, int heads, int kv_heads, int ctx) {
+                                                            int64_t wo_seq, int heads, int kv_heads, int nseq, int ctx, int* __restrict__ status) {
     gb_pdl_entry();
+    if (heads == 0 && blockIdx.x + blockIdx.y + blockIdx.z == 0 && threadIdx.x < 32) report_lens(lens, nseq, ctx, status);
     const int j = blockIdx.x * 256 + threadIdx.x, kh = blockIdx.y, s = blockIdx.z, group = heads / kv_heads;
     if (j >= checked_len(lens[s], ctx)) return;
     float x = 0.0f;
@@ -620,13 +626,13 @@ extern "C" int galois_b200_cache_attention_f32(galois_b200_ctx* ctx, const float
     if (heads > 65535 || (heads && (c.kv_heads == 0 || heads % c.kv_heads)))
         return gb_fail(ctx, GALOIS_B200_E_BROADCAST, "%s: %lld heads over %d key/value heads", what, (long long)heads, c.kv_heads);
     if (!isfinite(scale)) return gb_fail(ctx, GALOIS_B200_E_BADARG, "%s: scale is not finite", what);
-    if (heads == 0 || c.seqs == 0) return 0;
-    if (!q || !lens || !dst || !workspace) return gb_fail(ctx, GALOIS_B200_E_BADARG, "%s: null pointer", what);
+    if (c.seqs == 0 || (heads == 0 && !(weights && c.kv_heads))) return 0;
+    if (!lens || (heads && (!q || !dst || !workspace))) return gb_fail(ctx, GALOIS_B200_E_BADARG, "%s: null pointer", what);
     if (qd->nb[0] != 1 || dd->nb[0] != 1 || (uintptr_t)q % 16 || (uintptr_t)dst % 16 || (heads > 1 && (qd->nb[1] % 4 || dd->nb[1] % 4)) ||
         (c.seqs > 1 && (qd->nb[2] % 4 || dd->nb[2] % 4)) || (uintptr_t)lens % 4 || (uintptr_t)workspace % 16)
         return gb_fail(ctx, GALOIS_B200_E_LAYOUT, "%s: rows of q and dst must be contiguous, they and the workspace 16-byte aligned", what);
     if (!gb_injective(dd)) return gb_fail(ctx, GALOIS_B200_E_DST, "%s: rows of dst overlap", what);
-    const size_t qn = gb_span(qd, 4), dn = gb_span(dd, 4), ln = 4 * (size_t)c.seqs, need = layout(ctx, c, (int)heads, weights != nullptr).total * sizeof(float);
+    const size_t qn = gb_span(qd, 4), dn = gb_span(dd, 4), ln = 4 * (size_t)c.seqs, need = heads ? layout(ctx, c, (int)heads, weights != nullptr).total * sizeof(float) : 0;
     if (workspace_bytes < need) return gb_fail(ctx, GALOIS_B200_E_NOMEM, "%s: workspace of %zu bytes, %zu are needed", what, workspace_bytes, need);
     size_t wn = 0, won = 0;
     if (weights) {
@@ -655,9 +661,9 @@ extern "C" int galois_b200_cache_attention_f32(galois_b200_ctx* ctx, const float
     gb_on_device on(ctx);
     const layout L(ctx, c, (int)heads, weights != nullptr);
     float* ws = (float*)workspace;
-    float *final_stats = weights ? ws + L.final_stats : nullptr, *scores = weights ? ws + L.scores : nullptr;
+    float *final_stats = weights ? ws + L.final_stats : nullptr, *scores = weights ? ws + L.scores : nullptr;  // not used without heads
     const int group = (int)heads / c.kv_heads, tiles = (group + 7) / 8, rows = group < 8 ? group : 8;
-    if (c.ctx > 0) {  // else every length is 0
+    if (heads > 0 && c.ctx > 0) {  // else every length is 0
         CUtensorMap k_map, v_map;
         const uint64_t size[4] = {(uint64_t)c.head_dim, (uint64_t)c.ctx, (uint64_t)c.kv_heads, (uint64_t)c.seqs};
         // the stride of a dimension of one element means nothing, but has to be a valid one
@@ -675,13 +681,15 @@ extern "C" int galois_b200_cache_attention_f32(galois_b200_ctx* ctx, const float
     }
     // one sequence of 32 heads: 14.3 us with eight warps a head, 22.6 with one; 64 sequences of 32: 149.6 and 145.5
     const bool few = (int64_t)heads * c.seqs < 4 * ctx->sm_count;
-    auto join = c.head_dim == 64 ? (few ? cache_join_kernel<64, 8> : cache_join_kernel<64, 1>) : (few ? cache_join_kernel<128, 8> : cache_join_kernel<128, 1>);
-    GB_CUDA(ctx, gb_launch(ctx, join, dim3((unsigned)(few ? heads : (heads + 7) / 8), (unsigned)c.seqs), dim3(256), 0, lens, c.seqs, c.ctx, c.kv_heads, group,
-                           tiles, rows, ctx->sm_count * WARPS, ws + L.acc, ws + L.stats, dst, dd->nb[1], dd->nb[2], final_stats));
-    GB_LAUNCHED(ctx, "cache_join");
+    if (heads > 0) {
+        auto join = c.head_dim == 64 ? (few ? cache_join_kernel<64, 8> : cache_join_kernel<64, 1>) : (few ? cache_join_kernel<128, 8> : cache_join_kernel<128, 1>);
+        GB_CUDA(ctx, gb_launch(ctx, join, dim3((unsigned)(few ? heads : (heads + 7) / 8), (unsigned)c.seqs), dim3(256), 0, lens, c.seqs, c.ctx, c.kv_heads, group,
+                               tiles, rows, ctx->sm_count * WARPS, ws + L.acc, ws + L.stats, dst, dd->nb[1], dd->nb[2], final_stats, ctx->dev_status));
+        GB_LAUNCHED(ctx, "cache_join");
+    }
     if (weights && c.ctx) {
         GB_CUDA(ctx, gb_launch(ctx, cache_weights_kernel, dim3((unsigned)((c.ctx + 255) / 256), (unsigned)c.kv_heads, (unsigned)c.seqs), dim3(256), 0, lens, final_stats,
-                               scores, weights, wd->nb[1], wd->nb[2], weights_out, wod->nb[1], wod->nb[2], (int)heads, c.kv_heads, c.ctx));
+                               scores, weights, wd->nb[1], wd->nb[2], weights_out, wod->nb[1], wod->nb[2], (int)heads, c.kv_heads, c.seqs, c.ctx, ctx->dev_status));
         GB_LAUNCHED(ctx, "cache_weights");
     }
     return 0;

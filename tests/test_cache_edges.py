@@ -112,3 +112,31 @@ def test_cache_attention_over_infinite_values(dev, G, hd):
         rows = np.delete(x[s].astype(np.float64), np.r_[gone], axis=0)
         step = np.abs(rows).max() / 127 / 2  # what the 8 bits are off by, at most
         assert np.all(np.abs(got[s] - rows.mean(0)) <= step * 1.001)
+
+
+# ------------------------------------------------------------------------------------------------ no heads, long rows, large counts
+
+
+def test_weights_of_no_heads_are_the_weights_there_were(dev, G):
+    rng = np.random.default_rng(4)
+    cache = upload(G, random_cache(rng, 2, 3, 50, 64))
+    w, lens = rng.random((2, 3, 50)).astype(np.float32), np.array([50, 20], np.int32)
+    none = gb.Tensor.zeros((64, 0, 2), F32, G)
+    wo = put(G, np.full_like(w, 7))
+    ws = gb.Tensor.zeros((max(1, gb.galois_cache_attention_workspace(cache, 0, True) // 4),), F32, G)
+    gb.galois_cache_attention(none, cache, put(G, lens), none, 0.1, ws, weights=put(G, w), weights_out=wo)
+    dev.synchronize()
+    got = wo.to_numpy()
+    for s, n in enumerate(lens):
+        assert np.array_equal(got[s, :, :n], w[s, :, :n]) and np.all(got[s, :, n:] == 7)
+    gb.galois_cache_attention(none, cache, put(G, np.array([51, 20], np.int32)), none, 0.1, ws, weights=put(G, w), weights_out=wo)
+    reported(dev)
+
+
+def test_lengths_in_a_cache_without_rows(dev, G):
+    cache = gb.CacheQ8.zeros(64, 0, 2, 3, G)
+    q, o = put(G, np.ones((3, 2, 64), np.float32)), put(G, np.full((3, 2, 64), 3, np.float32))
+    ws = gb.Tensor.zeros((gb.galois_cache_attention_workspace(cache, 2) // 4,), F32, G)
+    gb.galois_cache_attention(q, cache, put(G, np.array([0, 1, 0], np.int32)), o, 0.1, ws)
+    reported(dev)
+    assert not o.to_numpy().any()
