@@ -29,8 +29,9 @@
 // Tiles of 128 keys with one buffer of logits and tiles of 64 with two, before values and keys shared slots: 378 and 383 us
 // on the first, 54.1 and 52.9 on the second, 10.2 and 8.8 on 300 tokens; 64 were taken for the shorter ones.  The shared slots: 375.
 //
-// A probability of 0 does not hide a value that is not finite: where a result is not finite, its rows are formed again by
-// the plain loop below, which reads nothing that a query does not see.
+// A probability of 0 does not hide a value that is not finite: where a result is not finite (or has left F16's range), its rows
+// are formed again by the plain loop below, which reads nothing that a query does not see.  That is a warp a row and a step a
+// key: a value that is not finite costs every later query of its heads so much (the loop took 50 ms for all of the 8192 tokens).
 #include "kv_cache_q8.cuh"
 
 #include "tcgen05.cuh"
@@ -473,7 +474,10 @@ __global__ void __launch_bounds__(THREADS, 1)
             const int head = two_heads ? x.head0 + s : x.head0;
             T* out = reinterpret_cast<T*>(p.out) + (int64_t)head * p.o_head + (int64_t)(x.q0 + at - row) * p.o_tok;  // row 0's
             T* to = out + (int64_t)row * p.o_tok;
-            uint32_t odd = 0;  // sign bit: a result's exponent is all ones
+            // The sign bit of `odd`: a result is not finite, or beyond what F16 rounds to its largest number.  (Means of F16 numbers lie
+            // within their range, but probabilities that were rounded up can pass their sum's 1.)
+            constexpr uint32_t END = sizeof(T) == 4 ? 0x7f800000u : 0x477ff000u;
+            uint32_t odd = 0;
 #pragma unroll
             for (int i = 0; i < HD / 32; i++) {
                 uint32_t o[32];
@@ -482,7 +486,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
                 for (int e = 0; e < 32; e++) {
                     o[e] = none ? 0u : __float_as_uint(__uint_as_float(o[e]) * inv);
-                    odd |= (o[e] & 0x7f800000u) + 0x00800000u;
+                    odd |= (o[e] & 0x7fffffffu) + (0x80000000u - END);
                 }
                 if (!live) continue;
                 if constexpr (sizeof(T) == 4) {
@@ -495,7 +499,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
             }
             tc_before_sync();
-            // rows whose result is not finite, by the plain loop
+            // such rows by the plain loop
             for (uint32_t rows = __ballot_sync(0xffffffffu, live && (odd >> 31)); rows; rows &= rows - 1) {
                 const int w = __ffs(rows) - 1, i = at - lane + w, key = i + x.nk - x.nq + 1;
                 prompt_row<HD, T>(p.q, p.k, p.v, x.q0 + i, x.k0, key, head, x.kh, p.scale, out + (int64_t)(row - lane + w) * p.o_tok);

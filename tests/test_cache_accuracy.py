@@ -195,3 +195,25 @@ def test_keys_of_zeros_under_a_factor_beyond_the_range_of_f32(dev, G):
     got = attend(dev, G, q, (kq, ks, vq, vs), [n], 1.0)
     want = (vq[0, 0, 1::2].astype(np.float64) * np.float64(vs[0, 0, 0])).mean(0)
     assert np.all(np.abs(got - want) <= 2.0**-16 * want)  # as step64 counts, without logits
+
+
+# ------------------------------------------------------------------------------------------------ prompts
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_prompt_results_at_the_end_of_f16(dev, G, hd):
+    """The mean of values that are all the largest F16 is that number, whichever way their probabilities were rounded."""
+    n = 101
+    q, k = np.full((1, 1, hd), 0, np.float16), np.zeros((n, 1, hd), np.float16)
+    q[0, 0, 0] = -1
+    k[1:, 0, 0] = 1
+    v = np.full((n, 1, hd), 65504, np.float16)
+    v[:, 0, 1::2] *= -1
+    scale = -float(np.log(0.5 + 2.0**-12 + 2.0**-19))  # probabilities of the others, next to where F16 rounds up
+    for kind in (np.float16, np.float32):
+        dst = put(G, np.zeros((1, 1, hd), kind))
+        gb.galois_prompt_attention(put(G, q), put(G, k), put(G, v), put(G, np.array([0, 1], np.int32)), put(G, np.array([0, n], np.int32)), dst, scale)
+        dev.synchronize()
+        got = dst.to_numpy().astype(np.float64)
+        assert np.all(np.isfinite(got))
+        assert np.all(np.abs(got - v[0].astype(np.float64)) <= 65504 * 2.0**-11 * 1.01)
