@@ -20,8 +20,9 @@
 // two runs of tokens of one head.  Tensor memory: for each query tile two buffers of logits, 2 x 64 columns, so that the
 // tensor cores form the next logits while the soft-max has these, and the results, head_dim columns; the probabilities (F16)
 // overwrite the first half of their logits and are the second product's operand from there.  The running maximum that
-// probabilities refer to is raised only when a row's maximum passes it by 2^8 (F16 holds what that leaves), so that the
-// results in tensor memory are rarely rescaled.
+// probabilities refer to is raised only when a row's maximum passes it by 2^7, so that the results in tensor memory are
+// rarely rescaled; probabilities are held times 2^7, 2^14 at most, so that F16 keeps 11 bits of them down to 2^-21 of the row's
+// largest and is off by 2^-32 of it below (their sum is f32's, and many small ones may count beside a large one).
 //
 // Measured (B200): 8192 tokens in three prompts, 32 heads over 8 x 128: 371 to 375 us, 0.49 of the measured matrix rate;
 // 2048 tokens, 32 heads x 128: 53 us.  A step (two query tiles x 64 keys) takes some 1960 cycles: the products alone 1240
@@ -414,7 +415,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 uint32_t pk[KT / 2];  // probabilities, pairs of F16
                 uint64_t sums[2];
                 auto exponentials = [&]() {
-                    const float shift = top == -INFINITY ? 0.0f : -top * c;
+                    const float shift = top == -INFINITY ? 0.0f : fmaf(-top, c, 7.0f);
                     const uint64_t cc = f2_pack(c, c), sh = f2_pack(shift, shift);
                     sums[0] = sums[1] = 0;
 #pragma unroll
@@ -432,7 +433,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 // Behind the first tile the maximum that probabilities refer to hardly ever moves, so they are formed with the
                 // one there is, beside the search for the tile's own; should it have to move after all, they are formed again.
                 if (j > 0) exponentials();
-                const bool raise = (most - top) * c > 8.0f || (most != most && top == top);  // also the first maximum of a row
+                const bool raise = (most - top) * c > 7.0f || (most != most && top == top);  // also the first maximum of a row
                 if (j == 0 || __any_sync(0xffffffffu, raise)) {
                     const float keep = raise ? ex2((top - most) * c) : 1.0f;
                     if (raise) top = most;

@@ -200,6 +200,33 @@ def test_keys_of_zeros_under_a_factor_beyond_the_range_of_f32(dev, G):
 # ------------------------------------------------------------------------------------------------ prompts
 
 
+@pytest.mark.parametrize("hd,heads", [(64, 2), (128, 1)])
+@pytest.mark.parametrize("gap", [8, 12, 14, 16])
+@pytest.mark.parametrize("first", [0, 100, 2999])
+def test_prompt_sink_of_values_near_zero(dev, G, hd, heads, gap, first):
+    """As above for prompts, whose probabilities are rounded to F16: 11 bits down to 2^-21 of the row's largest, below that to
+    multiples of 2^-31 of it."""
+    n, nq = 3000, 3
+    q = np.zeros((nq, heads, hd), np.float16)
+    q[:, :, 0] = gap
+    k, v = np.zeros((n, 1, hd), np.float16), np.ones((n, 1, hd), np.float16)
+    k[first, 0, 0], v[first] = 1, 0
+    dst = put(G, np.zeros(q.shape, np.float32))
+    gb.galois_prompt_attention(put(G, q), put(G, k), put(G, v), put(G, np.array([0, nq], np.int32)), put(G, np.array([0, n], np.int32)), dst, 1.0)
+    dev.synchronize()
+    got = dst.to_numpy().astype(np.float64)
+    for i in range(nq):
+        seen = n - nq + i + 1
+        x = q[i, 0, 0].astype(np.float64) * k[:seen, 0, 0].astype(np.float64)
+        e = np.exp(x - x.max())
+        mass = (e * v[:seen, 0, 0]).sum()
+        out = mass / e.sum()
+        # half a step of F16, of its smallest numbers at 2^7 of the largest; logits' constant and product 2 h |x|; sums of n terms
+        # in blocks of 64, cut off at 2 h of the largest (4 steps of 17 terms, then one a block), exponentials 8 h
+        tol = out * (2.0**-11 + (2 * gap * 1.45 * 2 + 136 + 2 * (n / 64) * 2 + 16) * 2.0**-24) + 2.0**-32 * (v[:seen, 0, 0] != 0).sum() / e.sum()
+        assert np.all(np.abs(got[i] - out) <= tol), (i, np.max(np.abs(got[i] - out) / out))
+
+
 @pytest.mark.parametrize("hd", [64, 128])
 def test_prompt_results_at_the_end_of_f16(dev, G, hd):
     """The mean of values that are all the largest F16 is that number, whichever way their probabilities were rounded."""
