@@ -384,7 +384,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const float c = fmaxf(fabsf(p.scale) * 1.4426950408889634f, 1e-30f);  // not 0: a masked logit stays below all others
         const bool flip = p.scale < 0.0f;
         uint32_t nt = 0, done = 0;  // bit b: parity of the next logits in buffer b; the next last but one, the next last products
-        for (int r = 0;; r++) {
+        for (int r = 0; fine; r++) {  // a wait that ran out ends it: the other roles' waits on this one then run out once each
             const int64_t u = unit_of_round(r);
             // The unit is looked up here and again for the results: what describes it does not stay in registers.
             f.start(p, span);
@@ -395,7 +395,8 @@ __global__ void __launch_bounds__(THREADS, 1)
             float top = -INFINITY, l = 0.0f;  // what the probabilities refer to, their sum
             for (int j = 0; j < mine; j++) {
                 const uint32_t b = j & 1, b_at = s_at + b * KT;
-                fine = fine && __all_sync(0xffffffffu, arrived(s_full + 2 * s + b, (nt >> b) & 1, progress));
+                fine = __all_sync(0xffffffffu, arrived(s_full + 2 * s + b, (nt >> b) & 1, progress));
+                if (!fine) break;
                 nt ^= 1u << b;
                 tc_after_sync();
                 float y[KT];
@@ -441,7 +442,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                     if (j > 0) {
                         // products j - 1 are done: logits j + 1 come after them, or else a barrier of their own says so
                         const bool ok = j + 1 < mine ? arrived(s_full + 2 * s + (b ^ 1), (nt >> (b ^ 1)) & 1, progress) : arrived(pv_done + 2 * s, done & 1, progress);
-                        fine = fine && __all_sync(0xffffffffu, ok);
+                        fine = __all_sync(0xffffffffu, ok);
+                        if (!fine) break;
                         tc_after_sync();
 #pragma unroll
                         for (int i = 0; i < HD / 32; i++) {
@@ -464,10 +466,11 @@ __global__ void __launch_bounds__(THREADS, 1)
                 if (lane == 0) mbar_arrive(p_ready + 2 * s + b);
             }
             // ---- results
+            if (!fine) break;
             f.start(p, span);
             x.find(p, f, u, units, span, two_heads);
             const int at = x.first + (two_heads ? 0 : s * PT) + row;
-            if (mine > 0) fine = fine && __all_sync(0xffffffffu, arrived(pv_done + 2 * s + 1, done >> 1, progress));
+            if (mine > 0) fine = __all_sync(0xffffffffu, arrived(pv_done + 2 * s + 1, done >> 1, progress));
             done ^= mine > 1 ? 3u : mine > 0 ? 2u : 0u;
             tc_after_sync();
             const bool none = top == -INFINITY, live = fine && at < x.nq;  // no key, or none that counts
