@@ -55,13 +55,18 @@ struct piece<__half> {
 // A CTA of 128 threads looks at `tile` packed tokens of one head, of the keys (z = 0) or the values (z = 1).  Each
 // token there that is the first new one of its block leads the block: the CTA takes all new rows of that block into
 // registers (16 bytes of a row a lane), finds the largest magnitude, settles the scale and writes.  A block has one
-// leader, so no two CTAs write the same rows or scale.
+// leader, so no two CTAs write the same rows or scale.  Sequences out of range are left out as a whole; the last column of the
+// grid reports them.
 template <typename T, int HD>
 __global__ void __launch_bounds__(128) cache_append_kernel(const T* __restrict__ k, int64_t k_head, int64_t k_tok, const T* __restrict__ v,
                                                            int64_t v_head, int64_t v_tok, const int32_t* __restrict__ starts,
                                                            const int32_t* __restrict__ pos, int nseq, int tokens, int tile, gb_cache_view c,
                                                            int* __restrict__ status) {
     gb_pdl_entry();
+    if (blockIdx.x == gridDim.x - 1) {
+        if (blockIdx.y + blockIdx.z == 0) gb_report_packed(starts, pos, nseq, tokens, c.ctx, status);
+        return;
+    }
     constexpr int V = piece<T>::N, W = V / 4, LPR = HD / V, RPP = 128 / LPR, N = GB_CACHE_BLOCK / RPP;  // numbers and words a lane, lanes a row, rows a pass, passes
     __shared__ uint32_t red[4];
     const int head = blockIdx.y, warp = threadIdx.x >> 5;
@@ -79,8 +84,7 @@ __global__ void __launch_bounds__(128) cache_append_kernel(const T* __restrict__
             t = begin;
             continue;
         }
-        if (begin < 0 || begin > t || end <= t || end > tokens || p0 < 0 || p0 > c.ctx - (end - begin)) {
-            if (threadIdx.x == 0) *status = GALOIS_B200_E_BADARG;  // nothing of this sequence is written
+        if (begin > t || end <= t || !gb_packed_ok(begin, end, p0, tokens, c.ctx)) {
             t = end > t ? end : t + 1;
             continue;
         }
@@ -172,6 +176,10 @@ __global__ void __launch_bounds__(128) cache_read_kernel(gb_cache_view c, const 
                                                          int tokens, T* __restrict__ k, int64_t k_head, int64_t k_tok, T* __restrict__ v,
                                                          int64_t v_head, int64_t v_tok, int* __restrict__ status) {
     gb_pdl_entry();
+    if (blockIdx.x == gridDim.x - 1) {
+        if (blockIdx.y + blockIdx.z == 0) gb_report_packed(starts, pos, nseq, tokens, c.ctx, status);
+        return;
+    }
     constexpr int V = 16 / sizeof(T), W = V / 4, LPR = HD / V, RPP = 128 / LPR, N = READ_ROWS / RPP;
     const int head = blockIdx.y, col = (threadIdx.x % LPR) * V;
     const int8_t* q = (blockIdx.z ? c.v : c.k) + head * c.head + col;
@@ -185,7 +193,7 @@ __global__ void __launch_bounds__(128) cache_read_kernel(gb_cache_view c, const 
     uint32_t w[N][W];
     float d[N];
     bool live[N];
-    if (s < nseq && begin >= 0 && begin <= tile && end >= tile + READ_ROWS && end <= tokens && p0 >= 0 && p0 <= c.ctx - (end - begin)) {
+    if (s < nseq && begin <= tile && end >= tile + READ_ROWS && gb_packed_ok(begin, end, p0, tokens, c.ctx)) {
         // all rows of one sequence
         const int p = p0 + (t0 - begin);
         const int8_t* from = q + s * c.seq + p * c.tok;
@@ -209,22 +217,17 @@ __global__ void __launch_bounds__(128) cache_read_kernel(gb_cache_view c, const 
             while (s < nseq && end <= t) {
                 if (++s < nseq) begin = end, end = starts[s + 1], p0 = pos[s];
             }
-            const bool front = s == 0 && begin > t && end >= begin && end <= tokens;  // of the first sequence
-            if (t < tokens && s < nseq && !front) {
-                if (begin < 0 || begin > t || end > tokens || p0 < 0 || p0 > c.ctx - (end - begin)) {
-                    *status = GALOIS_B200_E_BADARG;
+            if (t < tokens && s < nseq && begin <= t && gb_packed_ok(begin, end, p0, tokens, c.ctx)) {
+                const int p = p0 + (t - begin);
+                live[i] = true;
+                const int8_t* from = q + s * c.seq + p * c.tok;
+                if constexpr (W == 1) {
+                    w[i][0] = *reinterpret_cast<const uint32_t*>(from);
                 } else {
-                    const int p = p0 + (t - begin);
-                    live[i] = true;
-                    const int8_t* from = q + s * c.seq + p * c.tok;
-                    if constexpr (W == 1) {
-                        w[i][0] = *reinterpret_cast<const uint32_t*>(from);
-                    } else {
-                        const uint2 u = *reinterpret_cast<const uint2*>(from);
-                        w[i][0] = u.x, w[i][1] = u.y;
-                    }
-                    d[i] = scales[s * c.s_seq + p / GB_CACHE_BLOCK];
+                    const uint2 u = *reinterpret_cast<const uint2*>(from);
+                    w[i][0] = u.x, w[i][1] = u.y;
                 }
+                d[i] = scales[s * c.s_seq + p / GB_CACHE_BLOCK];
             }
         }
     }
@@ -486,7 +489,7 @@ int append(galois_b200_ctx* ctx, const char* what, const galois_b200_cache_q8* c
     // A CTA per token where most tokens lead a block of their own (single tokens of many sequences), else per 32.  With the
     // read back, one and 32 tokens a CTA: a token each of 48 sequences 10.8 and 54 us, 8 000 tokens of prompts 153 and 36 us.
     const int tile = (int64_t)nseq * 8 >= tokens ? 1 : GB_CACHE_BLOCK;
-    const dim3 grid((unsigned)((tokens + tile - 1) / tile), (unsigned)c.kv_heads, 2);
+    const dim3 grid((unsigned)((tokens + tile - 1) / tile + 1), (unsigned)c.kv_heads, 2);  // and a column that reports
     auto kern = c.head_dim == 64 ? cache_append_kernel<T, 64> : cache_append_kernel<T, 128>;
     GB_CUDA(ctx, gb_launch(ctx, kern, grid, dim3(128), 0, k, kd->nb[1], kd->nb[2], v, vd->nb[1], vd->nb[2], starts, pos, nseq, tokens, tile, c, ctx->dev_status));
     GB_LAUNCHED(ctx, what);
@@ -511,7 +514,7 @@ int read_rows(galois_b200_ctx* ctx, const char* what, const galois_b200_cache_q8
     const int tokens = (int)kd->ne[2];
     if (tokens == 0 || nseq == 0 || c.kv_heads == 0) return 0;
     gb_on_device on(ctx);
-    const dim3 grid((unsigned)((tokens + READ_ROWS - 1) / READ_ROWS), (unsigned)c.kv_heads, 2);
+    const dim3 grid((unsigned)((tokens + READ_ROWS - 1) / READ_ROWS + 1), (unsigned)c.kv_heads, 2);  // and a column that reports
     auto kern = c.head_dim == 64 ? cache_read_kernel<T, 64> : cache_read_kernel<T, 128>;
     GB_CUDA(ctx, gb_launch(ctx, kern, grid, dim3(128), 0, c, starts, pos, nseq, tokens, k, kd->nb[1], kd->nb[2], v, vd->nb[1], vd->nb[2], ctx->dev_status));
     GB_LAUNCHED(ctx, what);

@@ -72,6 +72,17 @@ __device__ __forceinline__ int gb_find_seq(const int32_t* __restrict__ starts, i
     return __reduce_add_sync(0xffffffffu, c);
 }
 
+// Whether packed rows begin .. end can be rows p0.. of a slot.  The position of a sequence without rows does not matter.
+__device__ __forceinline__ bool gb_packed_ok(int begin, int end, int p0, int tokens, int ctx) {
+    return begin >= 0 && end >= begin && end <= tokens && (end == begin || (p0 >= 0 && p0 <= ctx - (end - begin)));
+}
+// By one CTA of its own, which nothing waits for: says so if a sequence is out of range, whether or not a token lies in it.
+__device__ __forceinline__ void gb_report_packed(const int32_t* __restrict__ starts, const int32_t* __restrict__ pos, int nseq, int tokens, int ctx,
+                                                 int* __restrict__ status) {
+    for (int i = threadIdx.x; i < nseq; i += blockDim.x)
+        if (!gb_packed_ok(starts[i], starts[i + 1], pos[i], tokens, ctx)) *status = GALOIS_B200_E_BADARG;
+}
+
 // A quotient x / d is rounded to a whole number (half to even) by adding 1.5 * 2^23 to x * (1 / d): the sum's last bits are
 // the number.  1 / d is not exact, so it is taken a little too small and a little too large: where both give the same
 // number it is the exact quotient's, else a border k + 1/2 lies next to it and is compared with in full.

@@ -52,6 +52,39 @@ def test_what_is_out_of_range_is_said_to_be(dev, G, what):
     dev.synchronize()
 
 
+@pytest.mark.parametrize("starts,pos,fine", [
+    ([0, 5, 9999], [3, 0], [0]),       # no token lies in the second sequence
+    ([0, 5, 5, 6], [3, 0, 0], [0]),
+    ([0, 2, 5, 4], [3, 7, 0], [0, 1]),  # the last one's end lies in front of its start
+    ([0, 5, 5], [3, 999], [0, 1]),     # nothing is wanted of the second: its position does not matter
+])
+def test_sequences_without_tokens_of_their_own(dev, G, starts, pos, fine):
+    rng = np.random.default_rng(2)
+    seqs = len(pos)
+    parts = random_cache(rng, seqs, 2, 64, 64)
+    x = [rng.normal(0, 1, (5, 2, 64)).astype(np.float32) for _ in range(2)]
+    cache, want = upload(G, parts), [p.copy() for p in parts]
+    s, p = put(G, np.array(starts, np.int32)), put(G, np.array(pos, np.int32))
+    gb.galois_cache_append(put(G, x[0]), put(G, x[1]), s, p, cache)
+    bad = len(fine) < seqs
+    reported(dev) if bad else dev.synchronize()
+    for i in fine:
+        a, b = starts[i], starts[i + 1]
+        for h in range(2):
+            R.append(x[h][a:b], [0, b - a], [pos[i]], want[2 * h][i:i + 1], want[2 * h + 1][i:i + 1])
+    for got, w in zip(parts_of(cache, want), want):
+        assert np.array_equal(got, w)
+    outs = [put(G, np.full((5, 2, 64), 9, np.float32)) for _ in range(2)]
+    gb.galois_cache_read(cache, s, p, *outs)
+    reported(dev) if bad else dev.synchronize()
+    for h, out in enumerate(outs):
+        rows, expect = R.values(want[2 * h], want[2 * h + 1]).astype(np.float32), np.full((5, 2, 64), 9, np.float32)
+        for i in fine:
+            a, b = starts[i], starts[i + 1]
+            expect[a:b] = rows[i, :, pos[i]:pos[i] + b - a].transpose(1, 0, 2)
+        assert np.array_equal(out.to_numpy(), expect)
+
+
 def descending(seqs, at, rng):
     """Starts of `seqs` sequences of 3 to 70 tokens; those behind sequence `at` begin again from the front."""
     lens = rng.integers(3, 71, seqs)
