@@ -216,6 +216,7 @@ __global__ void __launch_bounds__(128) cache_read_kernel(gb_cache_view c, const 
             live[i] = false;
             while (s < nseq && end <= t) {
                 if (++s < nseq) begin = end, end = starts[s + 1], p0 = pos[s];
+                if (end < begin) s = nseq;  // as gb_find_seq has it
             }
             if (t < tokens && s < nseq && begin <= t && gb_packed_ok(begin, end, p0, tokens, c.ctx)) {
                 const int p = p0 + (t - begin);

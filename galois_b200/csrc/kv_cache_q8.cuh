@@ -63,13 +63,18 @@ int gb_prompt_attention_init(galois_b200_ctx* ctx);
 int gb_check_cache(galois_b200_ctx* ctx, const char* what, const galois_b200_cache_q8* cache, gb_cache_view* out);
 
 #ifdef __CUDACC__
-// The sequence that packed row t belongs to: the number of starts[1..n] that are <= t.  Called by a whole warp;
-// the loads of a warp are independent of each other, so a batch of 32 sequences costs one trip to memory where a
-// binary search costs five.
+// The sequence that packed row t belongs to: the first that ends behind t, n if there is none.  Where starts descend, that
+// sequence and all behind it have no rows (they could be others' too).  Called by a whole warp; the loads of a warp are
+// independent of each other, so a batch of 32 sequences costs one trip to memory where a binary search costs five.
 __device__ __forceinline__ int gb_find_seq(const int32_t* __restrict__ starts, int n, int t) {
-    int c = 0;
-    for (int i = threadIdx.x & 31; i < n; i += 32) c += starts[i + 1] <= t;
-    return __reduce_add_sync(0xffffffffu, c);
+    unsigned first = (unsigned)n, descent = (unsigned)n;
+    for (int i = threadIdx.x & 31; i < n; i += 32) {
+        const int begin = starts[i], end = starts[i + 1];
+        if (end > t) first = min(first, (unsigned)i);
+        if (end < begin) descent = min(descent, (unsigned)i);
+    }
+    first = __reduce_min_sync(0xffffffffu, first);
+    return first < __reduce_min_sync(0xffffffffu, descent) ? (int)first : n;
 }
 
 // Whether packed rows begin .. end can be rows p0.. of a slot.  The position of a sequence without rows does not matter.

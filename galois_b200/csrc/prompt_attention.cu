@@ -149,22 +149,28 @@ __device__ __forceinline__ bool arrived(uint64_t* bar, uint32_t parity, const vo
 }
 
 // What of a sequence's starts can be used: queries [q0, q0 + nq), keys [k0, k0 + nk); false if they are out of range.
-__device__ __forceinline__ bool sequence(const prompt_args& p, int s, int& q0, int& nq, int& k0, int& nk) {
+__device__ __forceinline__ bool sequence(const prompt_args& p, int s, int& q0, int& nq, int& k0, int& nk, bool& descends) {
     q0 = p.q_starts[s], k0 = p.k_starts[s];
     const int q1 = p.q_starts[s + 1], k1 = p.k_starts[s + 1];
-    const bool ok = q0 >= 0 && q1 >= q0 && q1 <= p.tq && k0 >= 0 && k1 >= k0 && k1 <= p.tk;
+    descends = q1 < q0 || k1 < k0;
+    const bool ok = q0 >= 0 && q1 <= p.tq && k0 >= 0 && k1 <= p.tk && !descends;
     nq = ok ? q1 - q0 : 0, nk = ok ? k1 - k0 : 0;
     return ok;
 }
 
 // Where the CTA's units lie.  Units are counted with the heads fastest and, within a sequence, the tiles that see most keys
-// first.  A warp keeps 32 sequences, a lane each, and goes forward.
+// first.  A warp keeps 32 sequences, a lane each, and goes forward.  Where starts descend, that sequence and all behind it are left
+// out: their rows could be others' too, and would be written by two CTAs.
 struct unit_finder {
     int s0, before, mine, upto, q0, nq, k0, nk;  // first sequence held, tiles before it; this lane's sequence
     __device__ __forceinline__ void load(const prompt_args& p, int span) {
         const int s = s0 + (threadIdx.x & 31);
+        bool descends = false;
         q0 = nq = k0 = nk = 0;
-        if (s < p.nseq) sequence(p, s, q0, nq, k0, nk);
+        if (s < p.nseq) sequence(p, s, q0, nq, k0, nk, descends);
+        const uint32_t descents = __ballot_sync(0xffffffffu, descends);
+        if (descents << (31 - (threadIdx.x & 31))) nq = nk = 0;  // here or in a lower lane
+        if (descents) s0 = p.nseq;                               // no more are loaded
         mine = upto = (nq + span - 1) / span;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -358,8 +364,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     } else if (warp == CLEARER) {
         if (blockIdx.x == 0) {
             int a, b, c, d;
+            bool e;
             for (int s = lane; s < p.nseq; s += 32)
-                if (!sequence(p, s, a, b, c, d)) *p.status = GALOIS_B200_E_BADARG;
+                if (!sequence(p, s, a, b, c, d, e)) *p.status = GALOIS_B200_E_BADARG;
         }
         int it = 0, nr = 0;
         for (int r = 0; fine && x.find(p, f, unit_of_round(r), units, span, two_heads); r++) {

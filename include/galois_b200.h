@@ -436,8 +436,9 @@ int galois_b200_decode_attention_f32(galois_b200_ctx* ctx, const galois_b200_dec
  * 64 or 128.  Rows (head_dim numbers) are contiguous and 16-byte aligned, other strides free; destinations may not
  * overlap operands except where stated.  Packed rows: tokens starts[s] <= t < starts[s + 1] of a {head_dim, heads,
  * tokens} tensor belong to sequence s (i32 on the device, nseq + 1 of them, ascending); rows behind the last
- * sequence are neither read nor written.  Starts, positions and lengths out of range: that sequence's part is left
- * out and the next synchronising call returns GALOIS_B200_E_BADARG.  `scale` is finite; logits that f32 cannot hold
+ * sequence are neither read nor written, nor rows in front of the first.  Starts, positions and lengths out of range: that
+ * sequence's part is left out (where starts descend, that of every sequence behind it as well; a length out of range
+ * counts as 0) and the next synchronising call returns GALOIS_B200_E_BADARG.  `scale` is finite; logits that f32 cannot hold
  * give what inf gives. */
 
 /* out_i = sum_j softmax_j(scale * q_i . k_j) v_j, where query i of a sequence with nq queries and nk keys sees the

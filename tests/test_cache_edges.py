@@ -94,6 +94,42 @@ def descending(seqs, at, rng):
     return starts.astype(np.int32), tokens
 
 
+@pytest.mark.parametrize("seqs,at", [(3, 1), (40, 20), (70, 33), (70, 31), (70, 32), (70, 64)])
+def test_starts_that_descend_leave_out_what_comes_behind(dev, G, seqs, at):
+    """Sequences that would share tokens are not served one over the other: from the first descent on all are left out."""
+    rng = np.random.default_rng(seqs + at)
+    starts, tokens = descending(seqs, at, rng)
+    parts = random_cache(rng, seqs, 1, 80, 64)
+    x = [rng.normal(0, 1, (tokens, 1, 64)).astype(np.float32) for _ in range(2)]
+    pos = rng.integers(0, 10, seqs).astype(np.int32)
+    cache, want = upload(G, parts), [p.copy() for p in parts]
+    s, p = put(G, starts), put(G, pos)
+    gb.galois_cache_append(put(G, x[0]), put(G, x[1]), s, p, cache)
+    reported(dev)
+    for h in range(2):
+        R.append(x[h], starts[:at + 1], pos[:at], want[2 * h][:at], want[2 * h + 1][:at])
+    for got, w in zip(parts_of(cache, want), want):
+        assert np.array_equal(got, w)
+    outs = [put(G, np.full((tokens, 1, 64), 9, np.float32)) for _ in range(2)]
+    gb.galois_cache_read(cache, s, p, *outs)
+    reported(dev)
+    n = int(starts[at])
+    for h, out in enumerate(outs):
+        rows, got = R.values(want[2 * h], want[2 * h + 1]).astype(np.float32), out.to_numpy()
+        assert np.all(got[n:] == 9)
+        for i in range(at):
+            a, b = starts[i], starts[i + 1]
+            assert np.array_equal(got[a:b], rows[i, :, pos[i]:pos[i] + b - a].transpose(1, 0, 2))
+    q, k, v = (rng.normal(0, 1, (tokens, 2 if i == 0 else 1, 64)).astype(np.float16) for i in range(3))
+    out, bound = R.prompt(q, k, v, starts[:at + 1], starts[:at + 1], 0.125)
+    dst = put(G, np.full(q.shape, 3, np.float32))
+    gb.galois_prompt_attention(put(G, q), put(G, k), put(G, v), s, s, dst, 0.125)
+    reported(dev)
+    got = dst.to_numpy()
+    assert np.all(got[n:] == 3)
+    assert np.all(np.abs(got[:n] - out[:n]) <= bound[:n])
+
+
 # ------------------------------------------------------------------------------------------------ numbers at the end of f32
 
 
