@@ -136,6 +136,8 @@ def galois_cache_read(cache: CacheQ8, starts: Tensor, pos: Tensor, k: Tensor, v:
 def galois_cache_attention_workspace(cache: CacheQ8, heads: int, weights: bool = False) -> int:
     """Bytes of workspace that galois_cache_attention wants for `heads` query heads."""
     ctx = _ctx_of(cache.k)
+    if not 0 <= heads <= 65535:  # the C argument has 32 bits
+        raise GError(f"galois_cache_attention_workspace: {heads} heads")
     need = C.c_size_t()
     rc = lib.galois_b200_cache_attention_workspace_bytes(ctx, cache._ref, heads, 1 if weights else 0, C.byref(need))
     _check(ctx, rc, "galois_cache_attention_workspace")
@@ -179,6 +181,9 @@ def galois_cache_evict(cache: CacheQ8, lens: Tensor, weights: Tensor, recent: in
         _want(index, _I32, "galois_cache_evict index")
     _ints(lens, cache.seqs, "galois_cache_evict lens")
     _ints(out_lens, cache.seqs, "galois_cache_evict out_lens")
+    if recent < 0:
+        raise GError(f"galois_cache_evict: {recent} recent rows")
+    recent = min(recent, out.ctx)  # no more are kept; the C argument has 32 bits
     rc = lib.galois_b200_cache_evict(ctx, cache._ref, lens.data_ptr(), weights.data_ptr(), weights.c_dim(), recent, out._ref, out_lens.data_ptr(), out_weights.data_ptr(),
                                      out_weights.c_dim(), index.data_ptr(), index.c_dim())
     _check(ctx, rc, "galois_cache_evict")

@@ -209,3 +209,19 @@ def test_lengths_in_a_cache_without_rows(dev, G):
     gb.galois_cache_attention(q, cache, put(G, np.array([0, 1, 0], np.int32)), o, 0.1, ws)
     reported(dev)
     assert not o.to_numpy().any()
+
+
+@pytest.mark.parametrize("recent,same", [(2**32, 40), (2**32 + 3, 40), (2**31, 40)])
+def test_a_count_of_recent_rows_beyond_32_bits(dev, G, recent, same):
+    rng = np.random.default_rng(5)
+    parts = random_cache(rng, 1, 1, 100, 64)
+    w, lens = rng.random((1, 1, 100)).astype(np.float32), np.array([100], np.int32)
+    cut = gb.CacheQ8.zeros(64, 40, 1, 1, G)
+    ol, ow, ix = put(G, np.zeros(1, np.int32)), put(G, np.zeros((1, 1, 40), np.float32)), put(G, np.zeros((1, 1, 40), np.int32))
+    gb.galois_cache_evict(upload(G, parts), put(G, lens), put(G, w), recent, cut, ol, ow, ix)
+    dev.synchronize()
+    assert np.array_equal(ix.to_numpy(), R.evict(*parts, lens, w, 40, same)[6])
+    with pytest.raises(GError):
+        gb.galois_cache_evict(upload(G, parts), put(G, lens), put(G, w), -(2**32), cut, ol, ow, ix)
+    with pytest.raises(GError):
+        gb.galois_cache_attention_workspace(cut, 2**32 + 4)
