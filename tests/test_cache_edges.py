@@ -225,3 +225,50 @@ def test_a_count_of_recent_rows_beyond_32_bits(dev, G, recent, same):
         gb.galois_cache_evict(upload(G, parts), put(G, lens), put(G, w), -(2**32), cut, ol, ow, ix)
     with pytest.raises(GError):
         gb.galois_cache_attention_workspace(cut, 2**32 + 4)
+
+
+# ------------------------------------------------------------------------------------------------ behind the library's own operators
+
+
+def test_two_threads_with_a_context_each(dev, G):
+    """The first calls of two contexts made from two threads at once."""
+    import threading
+
+    import torch
+
+    rng = np.random.default_rng(9)
+    lens = np.array([200, 90], np.int32)
+    parts = random_cache(rng, 2, 2, 200, 64)
+    q, k, v, qs, _ = prompt_inputs(rng, 64, 4, 2, [(200, 200), (90, 90)], 0)
+    q1 = rng.normal(0, 1, (2, 4, 64)).astype(np.float32)
+    places = [gb.CudaDevice(0, torch.cuda.Stream()) for _ in range(2)]
+    got, failed = [None, None], []
+
+    def work(i):
+        try:
+            P = gb.Device.Gpu(places[i])
+            cache, o, o1 = upload(P, parts), put(P, np.zeros(q.shape, np.float16)), put(P, np.zeros_like(q1))
+            ws = gb.Tensor.zeros((gb.galois_cache_attention_workspace(cache, 4) // 4,), F32, P)
+            t = [put(P, a) for a in (q, k, v, qs)]
+            q1t, lt = put(P, q1), put(P, lens)
+            torch.cuda.synchronize()
+            for _ in range(30):
+                gb.galois_prompt_attention(*t, t[3], o, 0.125)
+                gb.galois_cache_attention(q1t, cache, lt, o1, 0.125, ws)
+            places[i].synchronize()
+            got[i] = (o.to_numpy(), o1.to_numpy())
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for p in places:
+        p.close()
+    assert not failed, failed
+    out, bound = R.prompt(q, k, v, qs, qs, 0.125)
+    step, step_bound, _, _ = R.step(q1, *parts, lens, 0.125)
+    for o, o1 in got:
+        assert np.all(np.abs(o - out) <= f16_bound(out, bound)) and np.all(np.abs(o1 - step) <= step_bound)
