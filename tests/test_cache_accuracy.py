@@ -73,8 +73,11 @@ def close(got, out, tol):
     assert np.all(np.abs(got - out) <= tol), f"{worst:.3g} of the tolerance"
 
 
-@pytest.mark.parametrize("hd,heads,kv,lens", [(128, 1, 1, [33]), (128, 4, 1, [700, 32, 5]), (64, 16, 2, [513, 64]), (128, 10, 1, [96, 200]), (64, 3, 3, [2000])])
-def test_exact_logits(dev, G, hd, heads, kv, lens):
+EXACT = [(128, 1, 1, [33]), (128, 4, 1, [700, 32, 5]), (64, 16, 2, [513, 64]), (128, 10, 1, [96, 200]), (64, 3, 3, [2000])]
+SINKS = [(128, 32), (128, 33), (64, 700), (128, 8192)]
+
+
+def exact_inputs(hd, heads, kv, lens):
     """Query numbers of 14 bits and values without a sign: both halves of the query and of the probabilities have to count."""
     rng = np.random.default_rng(hd + heads)
     ctx, seqs = max(lens), len(lens)
@@ -84,15 +87,17 @@ def test_exact_logits(dev, G, hd, heads, kv, lens):
     vq = rng.integers(1, 128, (seqs, kv, ctx, hd)).astype(np.int8)
     ks = np.ones((seqs, kv, (ctx + 31) // 32), np.float32)
     vs = np.exp(rng.normal(-3, 1, ks.shape)).astype(np.float32)
-    scale = 2.0**-18  # logits of some +-6
-    out, tol = step64(q, kq, ks, vq, vs, lens, scale)
-    close(attend(dev, G, q, (kq, ks, vq, vs), lens, scale), out, tol)
+    return q, (kq, ks, vq, vs), 2.0**-18  # logits of some +-6
 
 
-@pytest.mark.parametrize("gap", [8, 10, 14, 17, 20, 25])
-@pytest.mark.parametrize("hd,n", [(128, 32), (128, 33), (64, 700), (128, 8192)])
-def test_a_sink_of_values_near_zero(dev, G, gap, hd, n):
-    """One row takes nearly all of the probability and has nothing to give: the result is what the others' small probabilities make."""
+@pytest.mark.parametrize("hd,heads,kv,lens", EXACT)
+def test_exact_logits(dev, G, hd, heads, kv, lens):
+    q, parts, scale = exact_inputs(hd, heads, kv, lens)
+    out, tol = step64(q, *parts, lens, scale)
+    close(attend(dev, G, q, parts, lens, scale), out, tol)
+
+
+def sink_inputs(gap, hd, n):
     rng = np.random.default_rng(gap + n)
     q = np.zeros((1, 2, hd), np.float32)
     q[0, 0, 0], q[0, 1, 0] = gap, gap - 3
@@ -102,8 +107,16 @@ def test_a_sink_of_values_near_zero(dev, G, gap, hd, n):
     kq[0, 0, at, 0], vq[0, 0, at] = 1, 0
     ks = np.ones((1, 1, (n + 31) // 32), np.float32)
     vs = np.exp(rng.normal(-3, 1, ks.shape)).astype(np.float32)
-    out, tol = step64(q, kq, ks, vq, vs, [n], 1.0)
-    close(attend(dev, G, q, (kq, ks, vq, vs), [n], 1.0), out, tol)
+    return q, (kq, ks, vq, vs)
+
+
+@pytest.mark.parametrize("gap", [8, 10, 14, 17, 20, 25])
+@pytest.mark.parametrize("hd,n", SINKS)
+def test_a_sink_of_values_near_zero(dev, G, gap, hd, n):
+    """One row takes nearly all of the probability and has nothing to give: the result is what the others' small probabilities make."""
+    q, parts = sink_inputs(gap, hd, n)
+    out, tol = step64(q, *parts, [n], 1.0)
+    close(attend(dev, G, q, parts, [n], 1.0), out, tol)
 
 
 def test_a_loud_block_that_has_no_weight(dev, G):
@@ -244,3 +257,18 @@ def test_prompt_results_at_the_end_of_f16(dev, G, hd):
         got = dst.to_numpy().astype(np.float64)
         assert np.all(np.isfinite(got))
         assert np.all(np.abs(got - v[0].astype(np.float64)) <= 65504 * 2.0**-11 * 1.01)
+
+
+def test_prompt_attention_is_the_same_every_time(dev, G):
+    rng = np.random.default_rng(9)
+    lens = [700, 3, 260, 1, 129]
+    n = sum(lens)
+    st = put(G, np.concatenate([[0], np.cumsum(lens)]).astype(np.int32))
+    q, k, v = (put(G, rng.normal(0, 2, (n, h, 128)).astype(np.float16)) for h in (8, 2, 2))
+    seen = set()
+    for _ in range(8):
+        dst = put(G, np.zeros((n, 8, 128), np.float32))
+        gb.galois_prompt_attention(q, k, v, st, st, dst, 0.3)
+        dev.synchronize()
+        seen.add(dst.to_numpy().tobytes())
+    assert len(seen) == 1

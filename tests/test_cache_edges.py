@@ -211,6 +211,35 @@ def test_lengths_in_a_cache_without_rows(dev, G):
     assert not o.to_numpy().any()
 
 
+@pytest.mark.parametrize("n,budget,recent", [(20000, 4097, 300), (8193, 8192, 1), (16384, 9000, 0), (17000, 16999, 16000)])
+@pytest.mark.parametrize("kind", ["steps", "equal", "odd"])
+def test_evict_of_more_rows_than_a_chunk(dev, G, n, budget, recent, kind):
+    rng = np.random.default_rng(n)
+    lens = np.array([n, n - 4000], np.int32)
+    parts = random_cache(rng, 2, 1, n, 64)
+    w = np.exp(rng.normal(0, 2, (2, 1, n))).astype(np.float32)
+    if kind == "steps":
+        w = (np.floor(w * 4) / 4).astype(np.float32)
+    elif kind == "equal":
+        w[:] = 0.25
+    else:
+        w -= 1
+        w.reshape(-1)[rng.integers(0, w.size, w.size // 4)] = rng.choice([np.nan, np.inf, -np.inf, 0.0, -0.0, 1e-45, -1e-45], w.size // 4)
+    cut_parts = [np.full((2, 1, budget, 64), 99, np.int8), np.full((2, 1, (budget + 31) // 32), 5, np.float32)] * 2
+    cut = upload(G, cut_parts)
+    ol, ow, ix = put(G, np.full(2, -7, np.int32)), put(G, np.full((2, 1, budget), 6, np.float32)), put(G, np.full((2, 1, budget), -1, np.int32))
+    gb.galois_cache_evict(upload(G, parts), put(G, lens), put(G, w), recent, cut, ol, ow, ix)
+    dev.synchronize()
+    want = R.evict(*parts, lens, w, budget, recent)
+    assert np.array_equal(ix.to_numpy(), want[6]) and np.array_equal(ol.to_numpy(), want[4])
+    got, got_w = parts_of(cut, cut_parts), ow.to_numpy()
+    for s in range(2):
+        m = want[4][s]
+        assert np.array_equal(got_w[s, :, :m], want[5][s, :, :m], equal_nan=True) and np.all(got_w[s, :, m:] == 6)
+        for i in (0, 2):
+            assert np.array_equal(got[i][s, :, :m], want[i][s, :, :m]) and np.all(got[i][s, :, m:] == 99)
+
+
 @pytest.mark.parametrize("recent,same", [(2**32, 40), (2**32 + 3, 40), (2**31, 40)])
 def test_a_count_of_recent_rows_beyond_32_bits(dev, G, recent, same):
     rng = np.random.default_rng(5)
@@ -227,7 +256,107 @@ def test_a_count_of_recent_rows_beyond_32_bits(dev, G, recent, same):
         gb.galois_cache_attention_workspace(cut, 2**32 + 4)
 
 
+# ------------------------------------------------------------------------------------------------ operands over one another
+
+
+@pytest.mark.parametrize("heads,kv", [(4, 4), (3, 3), (4, 2)])
+def test_prompt_attention_of_keys_that_all_heads_share(dev, G, heads, kv):
+    """Key/value heads, and tokens of the queries, at a stride of 0: operands may lie over one another, they are only read."""
+    rng = np.random.default_rng(6)
+    q, k, v, qs, ks = prompt_inputs(rng, 64, heads, 1, [(150, 150), (20, 70)], 0)
+    one = [put(G, x) for x in (k, v)]
+    shared = [t.view((64, kv, k.shape[0]), (1, 0, 64, 64 * k.shape[0])) for t in one]
+    out, bound = R.prompt(q, np.repeat(k, kv, 1), np.repeat(v, kv, 1), qs, ks, 0.125)
+    dst = put(G, np.zeros(q.shape, np.float32))
+    gb.galois_prompt_attention(put(G, q), *shared, put(G, qs), put(G, ks), dst, 0.125)
+    dev.synchronize()
+    assert np.all(np.abs(dst.to_numpy() - out) <= bound)
+
+
+def test_append_of_keys_that_all_heads_share(dev, G):
+    rng = np.random.default_rng(7)
+    x = [rng.normal(0, 1, (50, 1, 128)).astype(np.float32) for _ in range(2)]
+    shared = [put(G, a).view((128, 3, 50), (1, 0, 128, 128 * 50)) for a in x]
+    parts = random_cache(rng, 1, 3, 64, 128)
+    cache, want = upload(G, parts), [p.copy() for p in parts]
+    gb.galois_cache_append(*shared, put(G, np.array([0, 50], np.int32)), put(G, np.array([7], np.int32)), cache)
+    dev.synchronize()
+    for i in range(2):
+        R.append(np.repeat(x[i], 3, 1), [0, 50], [7], want[2 * i], want[2 * i + 1])
+    for got, w in zip(parts_of(cache, want), want):
+        assert np.array_equal(got, w)
+
+
 # ------------------------------------------------------------------------------------------------ behind the library's own operators
+
+
+def test_a_layer_s_attention_from_projections_to_tokens(dev, G, oracle):
+    """Q4_0 projections, rope, the copy to F16, prompt attention, append; then a token: projections, rope, append, attention over the
+    cache, output projection.  Each of the new operators is compared with its plain form on what the library's others gave it."""
+    rng = np.random.default_rng(8)
+    hd, heads, kv, lens, ctx = 64, 4, 2, [40, 25], 64
+    width, n = hd * heads, sum(lens)
+    scale = hd**-0.5
+
+    def weight(rows, seed):
+        w = oracle.quantize_q4_0(oracle.fill_normal(rows * width, seed, 0, 0.06).reshape(rows, width))
+        return gb.Tensor.from_raw(w, (width, rows), GGmlType.Q4_0, G)
+
+    wq, wk, wv, wo = weight(width, 1), weight(hd * kv, 2), weight(hd * kv, 3), weight(width, 4)
+    rope = gb.RopeCustomOption(n_dims=hd)
+
+    def project(w, x, count, positions):
+        """{head_dim, heads, tokens} of the projection, turned if positions are given."""
+        tokens, rows = x.dim().shape[1], count * hd
+        y = gb.Tensor.zeros((rows, tokens), F32, G)
+        gb.galois_matmul(w, x, y)
+        y = y.view((hd, count, tokens), (1, hd, rows, rows * tokens))
+        if positions is None:
+            return y
+        turned = gb.Tensor.zeros((hd, count, tokens), F32, G)
+        gb.galois_rope_custom(rope, y, positions, turned)
+        return turned
+
+    def half(x):
+        y = gb.Tensor.zeros(x.dim().shape[:3], F16, G)
+        gb.galois_cpy(x, y)
+        return y
+
+    x = put(G, rng.normal(0, 1, (n, width)).astype(np.float32))
+    at = put(G, np.concatenate([np.arange(m) for m in lens]).astype(np.int32))
+    q, k, v = half(project(wq, x, heads, at)), half(project(wk, x, kv, at)), half(project(wv, x, kv, None))
+    starts = R.starts_of(lens)
+    st, zero = put(G, starts), put(G, np.zeros(2, np.int32))
+    out = gb.Tensor.zeros((hd, heads, n), F32, G)
+    cache = gb.CacheQ8.zeros(hd, ctx, kv, 2, G)
+    gb.galois_prompt_attention(q, k, v, st, st, out, scale)
+    gb.galois_cache_append(k, v, st, zero, cache)
+    y = gb.Tensor.zeros((width, n), F32, G)
+    gb.galois_matmul(wo, out.view((width, n), (1, width, width * n, width * n)), y)
+    ref, bound = R.prompt(q.to_numpy(), k.to_numpy(), v.to_numpy(), starts, starts, scale)
+    assert np.abs(ref).max() > 0.1
+    assert np.all(np.abs(out.to_numpy() - ref) <= bound)
+    want = [np.zeros((2, kv, ctx, hd), np.int8), np.zeros((2, kv, ctx // 32), np.float32)]
+    want = want + [a.copy() for a in want]
+    R.append(k.to_numpy(), starts, [0, 0], want[0], want[1])
+    R.append(v.to_numpy(), starts, [0, 0], want[2], want[3])
+    ws = gb.Tensor.zeros((gb.galois_cache_attention_workspace(cache, heads) // 4,), F32, G)
+    one = put(G, np.arange(3, dtype=np.int32))
+    for t in range(3):
+        x1, now = put(G, rng.normal(0, 1, (2, width)).astype(np.float32)), np.array(lens, np.int32) + t
+        pos = put(G, now)
+        q1, k1, v1 = project(wq, x1, heads, pos), project(wk, x1, kv, pos), project(wv, x1, kv, None)
+        o1, y1 = gb.Tensor.zeros((hd, heads, 2), F32, G), gb.Tensor.zeros((width, 2), F32, G)
+        gb.galois_cache_append(k1, v1, one, pos, cache)
+        gb.galois_cache_attention(q1, cache, put(G, now + 1), o1, scale, ws)
+        gb.galois_matmul(wo, o1.view((width, 2), (1, width, 2 * width, 2 * width)), y1)
+        R.append(back(k1, (2, kv, hd)), np.arange(3), now, want[0], want[1])
+        R.append(back(v1, (2, kv, hd)), np.arange(3), now, want[2], want[3])
+        for got, w in zip(parts_of(cache, want), want):
+            assert np.array_equal(got, w)
+        ref, bound, _, _ = R.step(back(q1, (2, heads, hd)), *want, now + 1, scale)
+        assert np.all(np.abs(o1.to_numpy() - ref) <= bound)
+        assert np.all(np.isfinite(y1.to_numpy()))
 
 
 def test_two_threads_with_a_context_each(dev, G):
