@@ -31,11 +31,13 @@ namespace {
 //    the values, CW numbers of four rows, whose bytes are paired by permutes.  Which row and which chunk g and t stand
 //    for is chosen so that the eight lanes of a load's phase meet no bank of the swizzled tile twice.
 //
-// Measured (B200): 64 sequences of up to 8192 rows, 8 key/value heads x 128, groups of 4: 664 MB in 145 to 148 us, 4.5 TB/s,
-// 0.69 of the copy rate; one sequence of 2048 rows, 32 heads: 14.3 us with the joining launch.  No unit is full (with twelve warps:
-// issue 0.50, ALU 0.36, FMA 0.26, tensor cores 0.27): an MMA with the conversion of its operand takes 13 to 16 cycles of
-// a scheduler, the bare one 8.6.  Eight warps or twelve with shorter rings, in one run (before pieces were kept as means): the batch 145 and 141 us, one sequence
-// 13.9 and 15.5, 16 sequences of up to 4096 with weights 37.7 and 38.5; eight lose 2.5 % on the first and gain on the others.
+// Measured (B200): 64 sequences of up to 8192 rows, 8 key/value heads x 128, groups of 4: 664 MB in 140 to 151 us (one build, different
+// cards), 4.4 to 4.7 TB/s, 0.67 to 0.72 of the copy rate; one sequence of 2048 rows, 32 heads: 13.9 us with the joining launch; 16
+// sequences of up to 4096 rows with weights 39.4 us.  No unit is full (issue 0.53, ALU 0.40, FMA 0.32, tensor cores 0.30): an MMA with
+// the conversion of its operand takes 13 to 16 cycles of a scheduler, the bare one 8.6.  Probabilities relative to each block, with
+// lower halves of their own power of two, cost 2.4 % of the batch (143.4 us beside 146.8) over ones relative to the piece, which were off by
+// 2^-25 of the largest.  Eight warps or twelve with shorter rings, in one run of an earlier build: the batch 145 and 141 us, one
+// sequence 13.9 and 15.5, 16 sequences with weights 37.7 and 38.5; eight lose 2.5 % on the first and gain on the others.
 constexpr int WARPS = 8;
 constexpr int BLK = GB_CACHE_BLOCK;
 template <int HD>
@@ -679,7 +681,7 @@ extern "C" int galois_b200_cache_attention_f32(galois_b200_ctx* ctx, const float
                                dim3(WARPS * 32), c.head_dim == 64 ? ring<64>::TOTAL : ring<128>::TOTAL, a, k_map, v_map));
         GB_LAUNCHED(ctx, what);
     }
-    // one sequence of 32 heads: 14.3 us with eight warps a head, 22.6 with one; 64 sequences of 32: 149.6 and 145.5
+    // one sequence of 32 heads: 13.9 us with eight warps a head, 23.0 with one; 64 sequences of 32: 145.4 and 141.4
     const bool few = (int64_t)heads * c.seqs < 4 * ctx->sm_count;
     if (heads > 0) {
         auto join = c.head_dim == 64 ? (few ? cache_join_kernel<64, 8> : cache_join_kernel<64, 1>) : (few ? cache_join_kernel<128, 8> : cache_join_kernel<128, 1>);

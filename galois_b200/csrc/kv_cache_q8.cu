@@ -6,9 +6,10 @@
 // it grows the rows already held are brought to the new scale, q' = round(q d_held / d).  Both roundings are exact
 // (half to even), which makes the contents a function of the numbers alone, whatever the order or split of the calls'
 // work.  All move bytes and are meant to be bound by HBM (B200, 6.55 TB/s measured copy rate): 50 000 rows of 8 heads x 128
-// are read into F16 in 53 us (5.8 TB/s); 8 000 F16 tokens appended in 17.5 us (49 MB, 2.8 TB/s), held back by the instructions
-// of the rounding; 16 sequences of up to 8192 rows cut to 2048 in 43 us (134 MB of rows), some of it the
-// selection, whose passes over the digits wait for one another.  Few rows cost a launch.
+// are read into F16 in 53 us (5.8 TB/s); 8 000 F16 tokens appended in 15.4 us where they lie in L2 and 19.3 from HBM (49 MB, 2.5
+// TB/s; 0.71 of the issue slots, for the rounding, and each CTA's chain of look-up, load, maximum and store); 16 sequences of up
+// to 8192 rows cut to 2048 in 42 us (134 MB of rows), some of it the selection, whose passes over the digits wait for one
+// another.  Few rows cost a launch.
 #include "kv_cache_q8.cuh"
 
 #include <type_traits>
@@ -487,8 +488,10 @@ int append(galois_b200_ctx* ctx, const char* what, const galois_b200_cache_q8* c
     const int tokens = (int)kd->ne[2];
     if (tokens == 0 || nseq == 0 || c.kv_heads == 0) return 0;
     gb_on_device on(ctx);
-    // A CTA per token where most tokens lead a block of their own (single tokens of many sequences), else per 32.  With the
-    // read back, one and 32 tokens a CTA: a token each of 48 sequences 10.8 and 54 us, 8 000 tokens of prompts 153 and 36 us.
+    // A CTA per token where most tokens lead a block of their own (single tokens of many sequences), else per 32.  One and 32
+    // tokens a CTA: a token each of 48 sequences 5.8 and 36 us, 8 000 tokens of prompts 135 and 15.4 us.  The host knows only the
+    // mean, which misleads where many single tokens come with one long prompt: 47 of them with one of 512 take 11.8 and 37.5 us,
+    // and the rule takes the second.
     const int tile = (int64_t)nseq * 8 >= tokens ? 1 : GB_CACHE_BLOCK;
     const dim3 grid((unsigned)((tokens + tile - 1) / tile + 1), (unsigned)c.kv_heads, 2);  // and a column that reports
     auto kern = c.head_dim == 64 ? cache_append_kernel<T, 64> : cache_append_kernel<T, 128>;

@@ -24,15 +24,16 @@
 // rarely rescaled; probabilities are held times 2^7, 2^14 at most, so that F16 keeps 11 bits of them down to 2^-21 of the row's
 // largest and is off by 2^-32 of it below (their sum is f32's, and many small ones may count beside a large one).
 //
-// Measured (B200): 8192 tokens in three prompts, 32 heads over 8 x 128: 371 to 375 us, 0.49 of the measured matrix rate;
-// 2048 tokens, 32 heads x 128: 53 us.  A step (two query tiles x 64 keys) takes some 1960 cycles: the products alone 1240
+// Measured (B200): 8192 tokens in three prompts, 32 heads over 8 x 128: 366 to 374 us, 0.49 to 0.50 of the measured matrix rate;
+// 2048 tokens, 32 heads x 128: 52 to 53 us.  A step (two query tiles x 64 keys) takes some 1960 cycles: the products alone 1240
 // of them (logits of 64 keys take 48 cycles an MMA, of 128 keys 64), the issuing warp's loop all of them, a tile's soft-max 1700.
 // Tiles of 128 keys with one buffer of logits and tiles of 64 with two, before values and keys shared slots: 378 and 383 us
 // on the first, 54.1 and 52.9 on the second, 10.2 and 8.8 on 300 tokens; 64 were taken for the shorter ones.  The shared slots: 375.
 //
 // A probability of 0 does not hide a value that is not finite: where a result is not finite (or has left F16's range), its rows
 // are formed again by the plain loop below, which reads nothing that a query does not see.  That is a warp a row and a step a
-// key: a value that is not finite costs every later query of its heads so much (the loop took 50 ms for all of the 8192 tokens).
+// key, for the queries behind a value that is not finite and those whose last tile of keys holds it: one infinite value of one
+// head among the 8192 tokens costs 109 ms if it is the first prompt's first, 28 ms if it is the last.
 #include "kv_cache_q8.cuh"
 
 #include "tcgen05.cuh"

@@ -445,8 +445,9 @@ int galois_b200_decode_attention_f32(galois_b200_ctx* ctx, const galois_b200_dec
  * keys j <= i + nk - nq (causal; a prompt that continues nk - nq earlier tokens).  Queries that see no key give
  * zeros; keys that a query does not see do not touch its result, whatever they hold.  q, dst {head_dim, heads,
  * tokens}; k, v {head_dim, kv_heads, tokens}; q_starts and k_starts may be the same array.  q, k, v are F16, dst F16
- * or f32; logits, sums and the running maximum are f32, the probabilities are rounded to F16 for the second product
- * as galois_matmul rounds its f32 operand for an F16 one. */
+ * or f32; logits, sums and the running maximum are f32, the probabilities are rounded to F16 (11 bits down to 2^-21 of a
+ * row's largest, nothing below 2^-32) for the second product, for either dst.  A key or value that is not finite slows
+ * the queries that see it, and those next to them, down by a hundred times. */
 int galois_b200_prompt_attention_f16(galois_b200_ctx* ctx, const void* q, const galois_dim* qd, const void* k, const galois_dim* kd, const void* v,
                                      const galois_dim* vd, const int32_t* q_starts, const int32_t* k_starts, int nseq, void* dst,
                                      const galois_dim* dd, float scale);
@@ -484,7 +485,7 @@ int galois_b200_cache_read_f16(galois_b200_ctx* ctx, const galois_b200_cache_q8*
 /* One new token per slot over the first lens[s] rows of its cache: out = sum_j softmax_j(scale * q . k_j) v_j; a
  * length of 0 gives zeros.  q, dst f32 {head_dim, heads, sequences}.  With `weights` (f32 {ctx, kv_heads, sequences};
  * NULL for none, then weights_out is NULL too) weights_out[j] = weights[j] + the sum over the group's heads of the
- * probability of row j, for j < lens[s]; weights_out may be weights itself.  workspace:
+ * probability of row j, for j < lens[s]; weights_out may be weights itself, and with no query heads is what weights is.  workspace:
  * galois_b200_cache_attention_workspace_bytes(cache, heads, with_weights) bytes, 16-byte aligned, contents
  * irrelevant; calls that may run at the same time (graphs replayed on two streams) need one each. */
 int galois_b200_cache_attention_workspace_bytes(galois_b200_ctx* ctx, const galois_b200_cache_q8* cache, int heads, int with_weights,
