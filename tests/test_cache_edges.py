@@ -6,11 +6,11 @@ import pytest
 import cache_reference as R
 import galois_b200 as gb
 from galois_b200 import GError, GGmlType
-from test_cache import back, f16_bound, parts_of, prompt_inputs, put, random_cache, upload
+from test_cache import back, f16_bound, parts_of, prompt_inputs, put, random_cache, spread, upload
 
 pytestmark = pytest.mark.gpu
 
-I8, I32, F16, F32 = GGmlType.I8, GGmlType.I32, GGmlType.F16, GGmlType.F32
+I32, F16, F32 = GGmlType.I32, GGmlType.F16, GGmlType.F32
 F32_MAX = np.finfo(np.float32).max
 
 
@@ -401,3 +401,125 @@ def test_two_threads_with_a_context_each(dev, G):
     step, step_bound, _, _ = R.step(q1, *parts, lens, 0.125)
     for o, o1 in got:
         assert np.all(np.abs(o - out) <= f16_bound(out, bound)) and np.all(np.abs(o1 - step) <= step_bound)
+
+
+# ------------------------------------------------------------------------------------------------ strides, places, lengths, graphs
+
+
+@pytest.mark.parametrize("hd,kv,ctx,budget", [(128, 2, 300, 100), (64, 3, 90, 64)])
+def test_evict_between_strided_tensors(dev, G, hd, kv, ctx, budget):
+    """Heads slowest, rows apart, in everything that is read and written; what lies between the rows stays."""
+    rng = np.random.default_rng(10)
+    lens = np.array([ctx, ctx - 7, budget - 1], np.int32)
+    seqs, blocks = 3, (budget + 31) // 32
+    parts = random_cache(rng, seqs, kv, ctx, hd)
+    w = rng.random((seqs, kv, ctx)).astype(np.float32)
+    w.reshape(-1)[::7] = 0.5
+
+    def apart(x, pad):
+        return spread(G, x, (2, 0, 1, 3) if x.ndim == 4 else (1, 0, 2), pad)
+
+    cache = gb.CacheQ8(*(apart(p, 16 if p.ndim == 4 else 3)[0] for p in parts))
+    to = [np.full((seqs, kv, budget, hd), 99, np.int8), np.full((seqs, kv, blocks), 5, np.float32)] * 2
+    cut = [apart(x, 16 if x.ndim == 4 else 1) for x in to]
+    ow, ix, ol = apart(np.full((seqs, kv, budget), 6, np.float32), 5), apart(np.full((seqs, kv, budget), -1, np.int32), 2), put(G, np.zeros(seqs, np.int32))
+    gb.galois_cache_evict(cache, put(G, lens), apart(w, 1)[0], 9, gb.CacheQ8(*(t[0] for t in cut)), ol, ow[0], ix[0])
+    dev.synchronize()
+    want = R.evict(*parts, lens, w, budget, 9)
+    assert np.array_equal(back(ix[0], (seqs, kv, budget)), want[6]) and np.array_equal(ol.to_numpy(), want[4])
+    got, got_w = [back(t[0], x.shape) for t, x in zip(cut, to)], back(ow[0], (seqs, kv, budget))
+    for s in range(seqs):
+        m = want[4][s]
+        assert np.array_equal(got_w[s, :, :m], want[5][s, :, :m]) and np.all(got_w[s, :, m:] == 6)
+        for i in (0, 2):
+            assert np.array_equal(got[i][s, :, :m], want[i][s, :, :m]) and np.all(got[i][s, :, m:] == 99)
+            assert np.array_equal(got[i + 1][s, :, :(m + 31) // 32], want[i + 1][s, :, :(m + 31) // 32])
+    for view, whole, before in cut + [ow, ix]:
+        n = view.dim().shape[0]
+        assert np.array_equal(whole.to_numpy()[..., n:], before[..., n:], equal_nan=before.dtype.kind == "f")
+
+
+@pytest.mark.parametrize("heads,kv", [(4, 2), (3, 1)])
+def test_prompts_that_do_not_begin_with_the_first_row(dev, G, heads, kv):
+    rng = np.random.default_rng(11)
+    qs, ks = np.array([70, 200, 201, 260], np.int32), np.array([3, 140, 300, 400], np.int32)
+    q, k, v = (rng.normal(0, 1, (n, h, 64)).astype(np.float16) for n, h in ((300, heads), (450, kv), (450, kv)))
+    q[:70], q[260:] = np.nan, np.inf
+    for x in (k, v):
+        x[:3], x[400:] = np.nan, np.inf
+    out, bound = R.prompt(q, k, v, qs, ks, 0.125)
+    dst = put(G, np.full(q.shape, 3, np.float32))
+    gb.galois_prompt_attention(put(G, q), put(G, k), put(G, v), put(G, qs), put(G, ks), dst, 0.125)
+    dev.synchronize()
+    got = dst.to_numpy()
+    assert np.all(got[:70] == 3) and np.all(got[260:] == 3)
+    assert np.all(np.abs(got[70:260] - out[70:260]) <= bound[70:260])
+
+
+@pytest.mark.parametrize("hd,heads,kv,nq,nk", [(64, 2, 1, 3, 70001), (128, 1, 1, 130, 20000), (64, 3, 3, 1, 40000)])
+def test_prompts_behind_long_prefixes(dev, G, hd, heads, kv, nq, nk):
+    rng = np.random.default_rng(12)
+    q, k, v, qs, ks = prompt_inputs(rng, hd, heads, kv, [(nq, nk)], 0)
+    out, bound = R.prompt(q, k, v, qs, ks, hd**-0.5)
+    dst = put(G, np.full(q.shape, 3, np.float32))
+    gb.galois_prompt_attention(put(G, q), put(G, k), put(G, v), put(G, qs), put(G, ks), dst, hd**-0.5)
+    dev.synchronize()
+    assert np.all(np.abs(dst.to_numpy() - out) <= bound)
+
+
+@pytest.mark.parametrize("kind", [np.float32, np.float16])
+def test_append_of_numbers_that_are_not_finite_into_blocks_that_hold_rows(dev, G, kind):
+    rng = np.random.default_rng(13)
+    parts = random_cache(rng, 3, 2, 96, 64)
+    x = [rng.normal(0, 1, (60, 2, 64)).astype(kind) for _ in range(2)]
+    x[0][3, 0, 5], x[0][4, 1, 6], x[1][40, 0, 0], x[1][59, 1, 63] = np.nan, np.inf, -np.inf, np.nan
+    x[1][25:30] = np.nan
+    starts, pos = np.array([0, 10, 30, 60], np.int32), np.array([20, 31, 50], np.int32)
+    cache, want = upload(G, parts), [p.copy() for p in parts]
+    gb.galois_cache_append(put(G, x[0]), put(G, x[1]), put(G, starts), put(G, pos), cache)
+    dev.synchronize()
+    for i in range(2):
+        R.append(x[i], starts, pos, want[2 * i], want[2 * i + 1])
+    for got, w in zip(parts_of(cache, want), want):
+        assert np.array_equal(got, w)
+
+
+def test_two_graphs_replayed_at_once(dev, G):
+    """A graph of each of two contexts, with a workspace each, replayed on two streams."""
+    import torch
+
+    rng = np.random.default_rng(14)
+    lens = np.array([600, 1000], np.int32)
+    work = []
+    for _ in range(2):
+        stream = torch.cuda.Stream()
+        own = gb.CudaDevice(0, stream)
+        P = gb.Device.Gpu(own)
+        parts = random_cache(rng, 2, 2, 1000, 128)
+        q1, w = rng.normal(0, 1, (2, 8, 128)).astype(np.float32), rng.random((2, 2, 1000)).astype(np.float32)
+        cache, t, o, wt, wo = upload(P, parts), put(P, q1), put(P, np.zeros_like(q1)), put(P, w), put(P, np.zeros_like(w))
+        ws, lt = gb.Tensor.zeros((gb.galois_cache_attention_workspace(cache, 8, True) // 4,), F32, P), put(P, lens)
+        torch.cuda.synchronize()
+        gb.galois_cache_attention(t, cache, lt, o, 0.09, ws, weights=wt, weights_out=wo)
+        own.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            gb.galois_cache_attention(t, cache, lt, o, 0.09, ws, weights=wt, weights_out=wo)
+        work.append((own, stream, graph, o, wo, R.step(q1, *parts, lens, 0.09, w), (cache, t, lt, wt, ws)))  # what a graph reads lives as long
+    try:
+        for _ in range(20):
+            for _, stream, graph, *_ in work:
+                with torch.cuda.stream(stream):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for own, _, _, o, wo, (out, bound, ww, wb), _ in work:
+            own.synchronize()
+            assert np.all(np.abs(o.to_numpy() - out) <= bound)
+            got = wo.to_numpy()
+            for s, n in enumerate(lens):
+                assert np.all(np.abs(got[s, :, :n] - ww[s, :, :n]) <= wb[s, :, :n]) and not got[s, :, n:].any()
+    finally:
+        torch.cuda.synchronize()
+        for w_ in work:
+            w_[2].reset()
+            w_[0].close()
